@@ -20,7 +20,11 @@ ext = CUDAExtension(
     sources=["spark_sklearn_amd/ops/csrc/ska_ops.hip"],
     extra_compile_args={
         "cxx": ["-O3", "-std=c++17"],
-        "nvcc": ["-O3", "-std=c++17", "--offload-arch=gfx950"],
+        # packed fp32 instructions stay off: hipcc makes them from ordinary
+        # float code, and some of their forms have given wrong results
+        "nvcc": ["-O3", "-std=c++17", "--offload-arch=gfx950",
+                 "-Xclang", "-target-feature",
+                 "-Xclang", "-packed-fp32-ops"],
     },
 )
 
