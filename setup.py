@@ -17,7 +17,8 @@ from torch.utils.cpp_extension import BuildExtension, CUDAExtension  # noqa: E40
 
 ext = CUDAExtension(
     name="spark_sklearn_amd._hip_ops",
-    sources=["spark_sklearn_amd/ops/csrc/ska_ops.hip"],
+    sources=["spark_sklearn_amd/ops/csrc/ska_ops.hip",
+             "spark_sklearn_amd/ops/csrc/ska_grouped.hip"],
     extra_compile_args={
         "cxx": ["-O3", "-std=c++17"],
         # packed fp32 instructions stay off: hipcc makes them from ordinary

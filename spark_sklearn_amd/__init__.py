@@ -19,6 +19,8 @@ helpers that replace SparkContext.
 from .converter import Converter
 from .grid_search import GridSearchCV
 from .group_apply import gapply
+from .grouped_rows import (GroupPlan, combine_rows, gather_rows, group_rows,
+                           grouped_linear)
 from .keyed_models import KeyedEstimator, KeyedModel, SparkSklearnEstimator
 from .random_search import RandomizedSearchCV
 from .udt import CSRVectorUDT, DeviceCSRMatrix
@@ -31,6 +33,8 @@ __all__ = [
     "GridSearchCV", "RandomizedSearchCV", "Converter",
     "KeyedEstimator", "KeyedModel", "SparkSklearnEstimator",
     "gapply", "CSRVectorUDT", "DeviceCSRMatrix",
+    "GroupPlan", "group_rows", "gather_rows", "combine_rows",
+    "grouped_linear",
     "HipContext", "createLocalContext", "init_distributed",
     "enable_prometheus",
 ]

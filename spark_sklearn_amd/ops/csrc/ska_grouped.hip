@@ -1,0 +1,901 @@
+// Grouped-row operators -- MI355X (gfx950, CDNA4) only.
+//
+// Rows that belong to groups (the keys of a keyed model, the experts of a
+// routed layer): a stable sort of the rows' group ids, the rows' way into
+// group order and back, and the product of each group's run of rows with
+// that group's own weights.  M = T*k entries (row t has k ids); `slots` is a
+// permutation of the entries, the ones without a group last, so that an
+// entry is kept exactly when its slot is below offsets[G].
+//
+// No kernel trusts the values of offsets and slots for its addresses: an
+// offset is clamped to the rows there are, a slot outside them is skipped.
+
+#include <torch/extension.h>
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <tuple>
+
+namespace {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+hipStream_t stream_now() {
+  return at::cuda::getCurrentCUDAStream().stream();
+}
+
+void check_launch() {
+  hipError_t e = hipGetLastError();
+  TORCH_CHECK(e == hipSuccess, "HIP launch failed: ", hipGetErrorString(e));
+}
+
+template <typename T>
+__device__ __forceinline__ float to_f(T v) {
+  return (float)v;
+}
+
+__device__ __forceinline__ int clampi(int v, int lo, int hi) {
+  return v < lo ? lo : (v > hi ? hi : v);
+}
+
+// ---------------------------------------------------------------------------
+// group_rows: a stable counting sort by id.  An id outside [0, G) is the key
+// G, so that such entries come last, in their own order.
+// ---------------------------------------------------------------------------
+template <typename I>
+__device__ __forceinline__ int key_of(I id, int G) {
+  return (id < 0 || id >= (I)G) ? G : (int)id;
+}
+
+// The first position in keys[0, n) whose key is not below g.
+__device__ __forceinline__ int lower_bound(const int* keys, int n, int g) {
+  int lo = 0, hi = n;
+  while (lo < hi) {
+    int mid = (lo + hi) >> 1;
+    if (keys[mid] < g)
+      lo = mid + 1;
+    else
+      hi = mid;
+  }
+  return lo;
+}
+
+constexpr int kSmallEntries = 2048;
+constexpr int kSmallGroups = 65536;
+
+// Few entries: one block.  An entry's slot is the number of entries that go
+// before it, counted by comparing it with every other, four keys a read.
+template <typename I>
+__global__ __launch_bounds__(1024) void sort_small_kernel(
+    const I* __restrict__ ids, int M, int G, int* __restrict__ offsets,
+    int* __restrict__ slots, int* __restrict__ order) {
+  __shared__ int4 key4[kSmallEntries / 4];
+  __shared__ int sorted[kSmallEntries];
+  int* key = reinterpret_cast<int*>(key4);
+  const int tid = threadIdx.x;
+  const int M4 = (M + 3) >> 2;
+  for (int i = tid; i < M4 * 4; i += 1024)
+    key[i] = i < M ? key_of<I>(ids[i], G) : 0x7fffffff;
+  __syncthreads();
+  for (int i = tid; i < M; i += 1024) {
+    const int me = key[i];
+    int before = 0;
+    for (int q = 0; q < M4; ++q) {
+      const int4 v = key4[q];
+      const int j = q * 4;
+      before += (v.x < me || (v.x == me && j < i));
+      before += (v.y < me || (v.y == me && j + 1 < i));
+      before += (v.z < me || (v.z == me && j + 2 < i));
+      before += (v.w < me || (v.w == me && j + 3 < i));
+    }
+    slots[i] = before;
+    order[before] = i;
+    sorted[before] = me;
+  }
+  __syncthreads();
+  for (int g = tid; g <= G; g += 1024) offsets[g] = lower_bound(sorted, M, g);
+}
+
+// Many entries: passes over a digit of the key, low digit first.  One pass
+// sorts up to kBins keys; more groups take two.  A pass counts each block's
+// digits, sums the counts over the blocks before it, and places the entries.
+constexpr int kBins = 8192;
+constexpr int kSortWaves = 4;
+
+template <typename I, bool FIRST>
+__device__ __forceinline__ int sort_key(const I* ids, const int* keys, int G,
+                                        int i) {
+  return FIRST ? key_of<I>(ids[i], G) : keys[i];
+}
+
+template <typename I, bool FIRST>
+__global__ __launch_bounds__(256) void sort_count_kernel(
+    const I* __restrict__ ids, const int* __restrict__ keys, int M, int G,
+    int shift, int mask, int bins, int tile, int blocks,
+    int* __restrict__ table) {
+  extern __shared__ int count[];
+  for (int b = threadIdx.x; b < bins; b += 256) count[b] = 0;
+  __syncthreads();
+  const long first = (long)blockIdx.x * tile;
+  const int last = (int)min(first + tile, (long)M);
+  for (long i = first + threadIdx.x; i < last; i += 256)
+    atomicAdd(&count[(sort_key<I, FIRST>(ids, keys, G, (int)i) >> shift) &
+                     mask],
+              1);
+  __syncthreads();
+  for (int b = threadIdx.x; b < bins; b += 256)
+    table[(long)b * blocks + blockIdx.x] = count[b];
+}
+
+__device__ __forceinline__ int wave_scan(int v, int lane) {
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    int o = __shfl_up(v, d);
+    if (lane >= d) v += o;
+  }
+  return v;
+}
+
+// One wave a bin: its counts become the numbers of such entries in the
+// blocks before, and total[bin] their sum.
+__global__ __launch_bounds__(256) void sort_scan_kernel(
+    int bins, int blocks, int* __restrict__ table, int* __restrict__ total) {
+  const int lane = threadIdx.x & 63;
+  const int bin = blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (bin >= bins) return;
+  int* row = table + (long)bin * blocks;
+  int sum = 0;
+  for (int b = 0; b < blocks; b += 64) {
+    int v = b + lane < blocks ? row[b + lane] : 0;
+    int s = wave_scan(v, lane);
+    if (b + lane < blocks) row[b + lane] = sum + s - v;
+    sum += __shfl(s, 63);
+  }
+  if (lane == 0) total[bin] = sum;
+}
+
+// The bins' first positions; where one pass sorts, these are the offsets.
+__global__ __launch_bounds__(1024) void sort_base_kernel(
+    int bins, const int* __restrict__ total, int* __restrict__ base) {
+  __shared__ int wave_sum[16];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  int carry = 0;
+  for (int b = 0; b < bins; b += 1024) {
+    int v = b + tid < bins ? total[b + tid] : 0;
+    int s = wave_scan(v, lane);
+    if (lane == 63) wave_sum[wave] = s;
+    __syncthreads();
+    int before = carry;
+    for (int w = 0; w < wave; ++w) before += wave_sum[w];
+    if (b + tid < bins) base[b + tid] = before + s - v;
+    for (int w = 0; w < 16; ++w) carry += wave_sum[w];
+    __syncthreads();
+  }
+}
+
+// Places a block's entries: each wave owns a contiguous part of the block's
+// tile and a row of counters.  Among 64 entries a lane's place is the number
+// of lower lanes with its digit.
+template <typename I, bool FIRST, bool LAST>
+__global__ __launch_bounds__(256) void sort_place_kernel(
+    const I* __restrict__ ids, const int* __restrict__ keys,
+    const int* __restrict__ entries, int M, int G, int shift, int mask,
+    int bits, int bins, int tile, int blocks, const int* __restrict__ table,
+    const int* __restrict__ base, int* __restrict__ keys_out,
+    int* __restrict__ order, int* __restrict__ slots) {
+  extern __shared__ int place[];  // [kSortWaves][bins]
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  for (int b = threadIdx.x; b < bins * kSortWaves; b += 256) place[b] = 0;
+  __syncthreads();
+  const int part = tile / kSortWaves;
+  const long first = (long)blockIdx.x * tile + (long)wave * part;
+  const long last = min(first + part, (long)M);
+  int* mine = place + wave * bins;
+  for (long i = first + lane; i < last; i += 64)
+    atomicAdd(&mine[(sort_key<I, FIRST>(ids, keys, G, (int)i) >> shift) &
+                    mask],
+              1);
+  __syncthreads();
+  for (int b = threadIdx.x; b < bins; b += 256) {
+    int at = base[b] + table[(long)b * blocks + blockIdx.x];
+#pragma unroll
+    for (int w = 0; w < kSortWaves; ++w) {
+      int n = place[w * bins + b];
+      place[w * bins + b] = at;
+      at += n;
+    }
+  }
+  __syncthreads();
+  volatile int* at = mine;
+  for (long i0 = first; i0 < last; i0 += 64) {
+    const long i = i0 + lane;
+    const bool in = i < last;
+    const int key = in ? sort_key<I, FIRST>(ids, keys, G, (int)i) : 0;
+    const int digit = (key >> shift) & mask;
+    unsigned long long same = __ballot(in);
+    for (int b = 0; b < bits; ++b) {
+      const bool one = (digit >> b) & 1;
+      const unsigned long long set = __ballot(one);
+      same &= one ? set : ~set;
+    }
+    const unsigned long long below = same & ((1ull << lane) - 1);
+    const int rank = __popcll(below);
+    const int start = in ? at[digit] : 0;
+    __builtin_amdgcn_wave_barrier();
+    if (in && rank == 0) at[digit] = start + __popcll(same);
+    __builtin_amdgcn_wave_barrier();
+    if (in) {
+      const int pos = start + rank;
+      const int entry = FIRST ? (int)i : entries[i];
+      order[pos] = entry;
+      if (!LAST || !FIRST) keys_out[pos] = key;
+      if (LAST) slots[entry] = pos;
+    }
+  }
+}
+
+__global__ void sort_offsets_kernel(const int* __restrict__ keys, int M,
+                                    int G, int* __restrict__ offsets) {
+  for (long g = (long)blockIdx.x * blockDim.x + threadIdx.x; g <= G;
+       g += (long)gridDim.x * blockDim.x)
+    offsets[g] = lower_bound(keys, M, (int)g);
+}
+
+template <typename I>
+void sort_launch(const I* ids, int M, int G, int* offsets, int* slots,
+                 int* order, at::TensorOptions opt) {
+  hipStream_t s = stream_now();
+  if (M <= kSmallEntries && G <= kSmallGroups) {
+    sort_small_kernel<I><<<1, 1024, 0, s>>>(ids, M, G, offsets, slots, order);
+    check_launch();
+    return;
+  }
+  int bits = 1;
+  while ((G >> bits) != 0) ++bits;  // keys are 0 .. G
+  const bool one = G + 1 <= kBins;
+  const int digit = one ? bits : (bits + 1) / 2;
+  const int mask = (1 << digit) - 1;
+  // 2048 entries a block at least, 1024 blocks at most
+  int tile = 2048;
+  while ((long)tile * 1024 < M) tile *= 2;
+  const int blocks = (int)(((long)M + tile - 1) / tile);
+  const int bins = one ? G + 1 : 1 << digit;
+  at::Tensor table = at::empty({(int64_t)bins * blocks + 2 * bins}, opt);
+  int* tab = table.data_ptr<int>();
+  int* total = tab + (long)bins * blocks;
+  int* base = one ? offsets : total + bins;
+  at::Tensor pairs;
+  int *k0 = nullptr, *e0 = nullptr, *k1 = nullptr;
+  if (!one) {
+    pairs = at::empty({3 * (int64_t)M}, opt);
+    k0 = pairs.data_ptr<int>();
+    e0 = k0 + M;
+    k1 = e0 + M;
+  }
+  const size_t lds = (size_t)bins * 4;
+  auto step = [&](auto first, auto last, int shift) {
+    constexpr bool F = decltype(first)::value, L = decltype(last)::value;
+    sort_count_kernel<I, F><<<blocks, 256, lds, s>>>(
+        ids, k0, M, G, shift, mask, bins, tile, blocks, tab);
+    sort_scan_kernel<<<(bins + 3) / 4, 256, 0, s>>>(bins, blocks, tab, total);
+    sort_base_kernel<<<1, 1024, 0, s>>>(bins, total, base);
+    sort_place_kernel<I, F, L><<<blocks, 256, lds * kSortWaves, s>>>(
+        ids, k0, e0, M, G, shift, mask, digit, bins, tile, blocks, tab, base,
+        L ? k1 : k0, L ? order : e0, slots);
+    check_launch();
+  };
+  auto set_lds = [&](auto kern) {
+    hipError_t e = hipFuncSetAttribute(
+        reinterpret_cast<const void*>(kern),
+        hipFuncAttributeMaxDynamicSharedMemorySize, kBins * 4 * kSortWaves);
+    TORCH_CHECK(e == hipSuccess, "HIP error: ", hipGetErrorString(e));
+  };
+  if (one) {
+    set_lds(sort_place_kernel<I, true, true>);
+    step(std::true_type{}, std::true_type{}, 0);
+  } else {
+    set_lds(sort_place_kernel<I, true, false>);
+    set_lds(sort_place_kernel<I, false, true>);
+    step(std::true_type{}, std::false_type{}, 0);
+    step(std::false_type{}, std::true_type{}, digit);
+    sort_offsets_kernel<<<std::min(1024, (G + 256) / 256), 256, 0, s>>>(
+        k1, M, G, offsets);
+    check_launch();
+  }
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> group_rows(
+    const at::Tensor& ids_in, int64_t n_groups) {
+  TORCH_CHECK(ids_in.is_cuda(), "group_rows: ids must be on the GPU");
+  TORCH_CHECK(ids_in.dtype() == at::kInt || ids_in.dtype() == at::kLong,
+              "group_rows: ids must be int32 or int64");
+  TORCH_CHECK(n_groups >= 1 && n_groups < (1 << 24),
+              "group_rows: n_groups must be in [1, 2^24)");
+  TORCH_CHECK(ids_in.numel() < (1ll << 31), "group_rows: too many entries");
+  c10::cuda::CUDAGuard guard(ids_in.device());
+  at::Tensor ids = ids_in.contiguous();
+  auto opt = ids.options().dtype(at::kInt);
+  const int M = (int)ids.numel(), G = (int)n_groups;
+  at::Tensor slots = at::empty(ids.sizes(), opt);
+  at::Tensor order = at::empty({M}, opt);
+  if (M == 0) return {at::zeros({G + 1}, opt), slots, order};
+  at::Tensor offsets = at::empty({G + 1}, opt);
+  if (ids.dtype() == at::kInt)
+    sort_launch<int>(ids.data_ptr<int>(), M, G, offsets.data_ptr<int>(),
+                     slots.data_ptr<int>(), order.data_ptr<int>(), opt);
+  else
+    sort_launch<int64_t>(ids.data_ptr<int64_t>(), M, G,
+                         offsets.data_ptr<int>(), slots.data_ptr<int>(),
+                         order.data_ptr<int>(), opt);
+  return {offsets, slots, order};
+}
+
+// ---------------------------------------------------------------------------
+// Rows into group order and back.  `lanes` lanes (a power of two up to 64)
+// share a row and walk it in vectors of 16 bytes.  Rows of an odd width
+// start at odd addresses, which the loads and stores here may have; the
+// elements behind the last whole vector go one by one.
+// ---------------------------------------------------------------------------
+template <typename T>
+struct Vec {
+  static constexpr int N = 16 / sizeof(T);
+  T v[N];
+};
+
+template <typename T>
+__device__ __forceinline__ Vec<T> load_vec(const T* p, int n) {
+  Vec<T> r;
+  if (n >= Vec<T>::N) {
+    __builtin_memcpy(&r, p, 16);
+  } else {
+#pragma unroll
+    for (int i = 0; i < Vec<T>::N; ++i) r.v[i] = i < n ? p[i] : (T)0.f;
+  }
+  return r;
+}
+
+template <typename T>
+__device__ __forceinline__ void store_vec(T* p, const Vec<T>& r, int n) {
+  if (n >= Vec<T>::N) {
+    __builtin_memcpy(p, &r, 16);
+  } else {
+#pragma unroll
+    for (int i = 0; i < Vec<T>::N; ++i)
+      if (i < n) p[i] = r.v[i];
+  }
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void gather_kernel(
+    const T* __restrict__ x, long x_pitch, const int* __restrict__ slots,
+    const int* __restrict__ kept_end, int T_rows, int k, int F, int lanes,
+    T* __restrict__ out) {
+  const int per = 256 / lanes;
+  const int t = blockIdx.x * per + threadIdx.x / lanes;
+  if (t >= T_rows) return;
+  const int M = T_rows * k;
+  const int S = clampi(*kept_end, 0, M);
+  constexpr int V = Vec<T>::N;
+  const T* src = x + (long)t * x_pitch;
+  for (int c = (threadIdx.x % lanes) * V; c < F; c += lanes * V) {
+    const Vec<T> v = load_vec(src + c, F - c);
+    for (int j = 0; j < k; ++j) {
+      const int s = slots[(long)t * k + j];
+      if ((unsigned)s >= (unsigned)M) continue;
+      Vec<T> w = v;
+      if (s >= S) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) w.v[i] = (T)0.f;
+      }
+      store_vec(out + (long)s * F + c, w, F - c);
+    }
+  }
+}
+
+// y[t] = sum over the kept entries of w[t, j] * rows[slots[t, j]], in the
+// order of j and in 32 bits.  W = void: no weights.
+template <typename T, typename W>
+__global__ __launch_bounds__(256) void combine_kernel(
+    const T* __restrict__ rows, long pitch, const int* __restrict__ slots,
+    const int* __restrict__ kept_end, const W* __restrict__ weights,
+    int T_rows, int k, int F, int lanes, T* __restrict__ y) {
+  const int per = 256 / lanes;
+  const int t = blockIdx.x * per + threadIdx.x / lanes;
+  if (t >= T_rows) return;
+  const int S = clampi(*kept_end, 0, T_rows * k);
+  constexpr int V = Vec<T>::N;
+  for (int c = (threadIdx.x % lanes) * V; c < F; c += lanes * V) {
+    float acc[V] = {};
+    for (int j = 0; j < k; ++j) {
+      const int s = slots[(long)t * k + j];
+      if ((unsigned)s >= (unsigned)S) continue;
+      const float w = weights ? (float)weights[(long)t * k + j] : 1.f;
+      const Vec<T> v = load_vec(rows + (long)s * pitch + c, F - c);
+#pragma unroll
+      for (int i = 0; i < V; ++i) acc[i] += w * to_f(v.v[i]);
+    }
+    Vec<T> o;
+#pragma unroll
+    for (int i = 0; i < V; ++i) o.v[i] = (T)acc[i];
+    store_vec(y + (long)t * F + c, o, F - c);
+  }
+}
+
+// Backward of combine, in row order: dy[t] is read once, each of its k rows
+// once; drows (where asked for) and the dot products leave with them.
+template <typename T, typename W>
+__global__ __launch_bounds__(256) void combine_back_kernel(
+    const T* __restrict__ dy, long dy_pitch, const T* __restrict__ rows,
+    long pitch, const int* __restrict__ slots,
+    const int* __restrict__ kept_end, const W* __restrict__ weights,
+    int T_rows, int k, int F, int lanes, T* __restrict__ drows,
+    W* __restrict__ dw) {
+  const int per = 256 / lanes;
+  const int t = blockIdx.x * per + threadIdx.x / lanes;
+  const bool in = t < T_rows;
+  const int M = T_rows * k;
+  const int S = clampi(*kept_end, 0, M);
+  constexpr int V = Vec<T>::N;
+  const int lane = threadIdx.x % lanes;
+  for (int j = 0; j < k; ++j) {
+    const int s = in ? slots[(long)t * k + j] : -1;
+    const bool kept = (unsigned)s < (unsigned)S;
+    const float w =
+        !kept ? 0.f : (weights ? (float)weights[(long)t * k + j] : 1.f);
+    float dot = 0.f;
+    if ((unsigned)s < (unsigned)M) {
+      for (int c = lane * V; c < F; c += lanes * V) {
+        const Vec<T> d = load_vec(dy + (long)t * dy_pitch + c, F - c);
+        if (dw && kept) {
+          const Vec<T> r = load_vec(rows + (long)s * pitch + c, F - c);
+#pragma unroll
+          for (int i = 0; i < V; ++i) dot += to_f(d.v[i]) * to_f(r.v[i]);
+        }
+        if (drows) {
+          Vec<T> o;
+#pragma unroll
+          for (int i = 0; i < V; ++i)
+            o.v[i] = kept ? (T)(w * to_f(d.v[i])) : (T)0.f;
+          store_vec(drows + (long)s * F + c, o, F - c);
+        }
+      }
+    }
+    if (dw) {
+      for (int d = lanes >> 1; d > 0; d >>= 1) dot += __shfl_xor(dot, d);
+      if (in && lane == 0) dw[(long)t * k + j] = (W)dot;
+    }
+  }
+}
+
+int lanes_for(int F, int vec) {
+  int lanes = 1;
+  while (lanes < 64 && lanes * vec < F) lanes *= 2;
+  return lanes;
+}
+
+#define SKA_TYPES(dtype, ...)                                             \
+  [&] {                                                                   \
+    if ((dtype) == at::kFloat) {                                          \
+      using T = float;                                                    \
+      return __VA_ARGS__();                                               \
+    }                                                                     \
+    if ((dtype) == at::kBFloat16) {                                       \
+      using T = __bf16;                                                   \
+      return __VA_ARGS__();                                               \
+    }                                                                     \
+    if ((dtype) == at::kHalf) {                                           \
+      using T = _Float16;                                                 \
+      return __VA_ARGS__();                                               \
+    }                                                                     \
+    TORCH_CHECK(false, "rows must be float32, bfloat16 or float16");      \
+  }()
+
+template <typename T>
+T* ptr(const at::Tensor& t) {
+  return reinterpret_cast<T*>(t.data_ptr());
+}
+
+// A matrix whose rows may lie apart but are contiguous in themselves.
+at::Tensor packed_rows(const at::Tensor& t) {
+  if (t.size(0) == 0 || t.size(1) == 0) return t;
+  const bool fits = (t.size(1) == 1 || t.stride(1) == 1) &&
+                    (t.size(0) == 1 || t.stride(0) >= t.size(1));
+  return fits ? t : t.contiguous();
+}
+
+void check_plan(const at::Tensor& x, const at::Tensor& offsets,
+                const at::Tensor& slots) {
+  TORCH_CHECK(x.is_cuda() && x.dim() == 2, "rows must be a GPU matrix");
+  TORCH_CHECK(offsets.dtype() == at::kInt && offsets.dim() == 1 &&
+                  offsets.numel() >= 2 && offsets.is_contiguous() &&
+                  offsets.device() == x.device(),
+              "offsets must be contiguous int32 [G + 1] on the rows' device");
+  TORCH_CHECK(slots.dtype() == at::kInt && slots.dim() == 2 &&
+                  slots.is_contiguous() && slots.device() == x.device() &&
+                  slots.numel() < (1ll << 31),
+              "slots must be contiguous int32 [T, k] on the rows' device");
+  TORCH_CHECK(x.size(1) < (1ll << 31) - 4096, "rows are too wide");
+}
+
+at::Tensor gather_rows(const at::Tensor& x_in, const at::Tensor& offsets,
+                       const at::Tensor& slots) {
+  check_plan(x_in, offsets, slots);
+  TORCH_CHECK(x_in.size(0) == slots.size(0), "one row for each of slots'");
+  c10::cuda::CUDAGuard guard(x_in.device());
+  at::Tensor x = packed_rows(x_in);
+  const int T_rows = (int)x.size(0), F = (int)x.size(1);
+  const int k = (int)slots.size(1);
+  at::Tensor out = at::empty({(int64_t)T_rows * k, F}, x.options());
+  if (out.numel() == 0) return out;
+  SKA_TYPES(x.scalar_type(), [&] {
+    const int lanes = lanes_for(F, Vec<T>::N), per = 256 / lanes;
+    gather_kernel<T><<<(T_rows + per - 1) / per, 256, 0, stream_now()>>>(
+        ptr<T>(x), x.stride(0), slots.data_ptr<int>(),
+        offsets.data_ptr<int>() + offsets.numel() - 1, T_rows, k, F, lanes,
+        ptr<T>(out));
+    check_launch();
+  });
+  return out;
+}
+
+void check_weights(const at::Tensor& rows, const at::Tensor& slots,
+                   const c10::optional<at::Tensor>& w) {
+  if (!w) return;
+  TORCH_CHECK(w->device() == rows.device() && w->sizes() == slots.sizes() &&
+                  w->is_contiguous(),
+              "weights must be contiguous and of the slots' shape");
+  TORCH_CHECK(w->dtype() == at::kFloat || w->dtype() == rows.dtype(),
+              "weights must be float32 or of the rows' type");
+}
+
+at::Tensor combine_rows(const at::Tensor& rows_in, const at::Tensor& offsets,
+                        const at::Tensor& slots,
+                        const c10::optional<at::Tensor>& weights) {
+  check_plan(rows_in, offsets, slots);
+  check_weights(rows_in, slots, weights);
+  TORCH_CHECK(rows_in.size(0) == slots.numel(), "one row for each slot");
+  c10::cuda::CUDAGuard guard(rows_in.device());
+  at::Tensor rows = packed_rows(rows_in);
+  const int T_rows = (int)slots.size(0), k = (int)slots.size(1);
+  const int F = (int)rows.size(1);
+  at::Tensor y = at::empty({T_rows, F}, rows.options());
+  if (y.numel() == 0) return y;
+  if (k == 0) return y.zero_();
+  SKA_TYPES(rows.scalar_type(), [&] {
+    const int lanes = lanes_for(F, Vec<T>::N), per = 256 / lanes;
+    const int blocks = (T_rows + per - 1) / per;
+    const int* end = offsets.data_ptr<int>() + offsets.numel() - 1;
+    if (!weights || weights->dtype() == at::kFloat)
+      combine_kernel<T, float><<<blocks, 256, 0, stream_now()>>>(
+          ptr<T>(rows), rows.stride(0), slots.data_ptr<int>(), end,
+          weights ? weights->data_ptr<float>() : nullptr, T_rows, k, F, lanes,
+          ptr<T>(y));
+    else
+      combine_kernel<T, T><<<blocks, 256, 0, stream_now()>>>(
+          ptr<T>(rows), rows.stride(0), slots.data_ptr<int>(), end,
+          ptr<T>(*weights), T_rows, k, F, lanes, ptr<T>(y));
+    check_launch();
+  });
+  return y;
+}
+
+// (drows, dw); one that is not asked for comes back undefined.
+std::tuple<c10::optional<at::Tensor>, c10::optional<at::Tensor>>
+combine_rows_backward(const at::Tensor& dy_in, const at::Tensor& rows_in,
+                      const at::Tensor& offsets, const at::Tensor& slots,
+                      const c10::optional<at::Tensor>& weights,
+                      bool need_rows, bool need_weights) {
+  check_plan(dy_in, offsets, slots);
+  check_weights(dy_in, slots, weights);
+  TORCH_CHECK(dy_in.size(0) == slots.size(0), "one gradient row a row");
+  TORCH_CHECK(!need_weights || weights, "no weights to differentiate");
+  if (need_weights)
+    TORCH_CHECK(rows_in.dim() == 2 && rows_in.size(0) == slots.numel() &&
+                    rows_in.size(1) == dy_in.size(1) &&
+                    rows_in.dtype() == dy_in.dtype() &&
+                    rows_in.device() == dy_in.device(),
+                "rows must be [T * k, F] like the gradient");
+  c10::cuda::CUDAGuard guard(dy_in.device());
+  at::Tensor dy = packed_rows(dy_in);
+  at::Tensor rows = need_weights ? packed_rows(rows_in) : dy;
+  const int T_rows = (int)slots.size(0), k = (int)slots.size(1);
+  const int F = (int)dy.size(1);
+  c10::optional<at::Tensor> drows, dw;
+  if (need_rows)
+    drows = at::empty({(int64_t)T_rows * k, F}, dy.options());
+  if (need_weights) dw = at::empty(slots.sizes(), weights->options());
+  if (slots.numel() == 0 || (!need_rows && !need_weights)) return {drows, dw};
+  if (F == 0) {
+    if (dw) dw->zero_();
+    return {drows, dw};
+  }
+  SKA_TYPES(dy.scalar_type(), [&] {
+    const int lanes = lanes_for(F, Vec<T>::N), per = 256 / lanes;
+    const int blocks = (T_rows + per - 1) / per;
+    const int* end = offsets.data_ptr<int>() + offsets.numel() - 1;
+    T* dr = drows ? ptr<T>(*drows) : nullptr;
+    if (!weights || weights->dtype() == at::kFloat)
+      combine_back_kernel<T, float><<<blocks, 256, 0, stream_now()>>>(
+          ptr<T>(dy), dy.stride(0), ptr<T>(rows), rows.stride(0),
+          slots.data_ptr<int>(), end,
+          weights ? weights->data_ptr<float>() : nullptr, T_rows, k, F, lanes,
+          dr, dw ? dw->data_ptr<float>() : nullptr);
+    else
+      combine_back_kernel<T, T><<<blocks, 256, 0, stream_now()>>>(
+          ptr<T>(dy), dy.stride(0), ptr<T>(rows), rows.stride(0),
+          slots.data_ptr<int>(), end, ptr<T>(*weights), T_rows, k, F, lanes,
+          dr, dw ? ptr<T>(*dw) : nullptr);
+    check_launch();
+  });
+  return {drows, dw};
+}
+
+// ---------------------------------------------------------------------------
+// Grouped products.  Row tiles are cut inside each group.  Tile i is found
+// from the offsets alone: group g's first tile has the index
+// floor(offsets[g] / BM) + g, which leaves every group room for its tiles
+// (ceil(n / BM) <= floor((a + n) / BM) - floor(a / BM) + 1), so the grid needs
+// no count from the device.  The rows behind the last group are a group of
+// their own, whose outputs are zero.
+// ---------------------------------------------------------------------------
+struct Segment {
+  int group, first, end;  // first >= end: nothing to do
+};
+
+__device__ __forceinline__ int edge(const int* offsets, int g, int G, int M) {
+  return g <= 0 ? 0 : (g > G ? M : clampi(offsets[g], 0, M));
+}
+
+template <int BM>
+__device__ __forceinline__ Segment find_segment(const int* offsets, int G,
+                                                int M, int tile) {
+  int lo = 0, hi = G + 1;  // the last group whose first tile is not behind
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (edge(offsets, mid, G, M) / BM + mid <= tile)
+      lo = mid;
+    else
+      hi = mid;
+  }
+  const int start = edge(offsets, lo, G, M);
+  const int end = edge(offsets, lo + 1, G, M);
+  const long first = start + (long)(tile - (start / BM + lo)) * BM;
+  return {lo, (int)min(first, (long)end), end};
+}
+
+// The plain tile: 64 x 64 outputs, 32 steps of the contraction at a time in
+// 32 bits through LDS, v_mfma_f32_16x16x4_f32.  Operands have any strides.
+constexpr int kTile = 64, kDepth = 32, kPitch = 36;
+
+template <typename T>
+__device__ __forceinline__ void load_tile(const T* src, long s_row, long s_k,
+                                          int rows, int depth,
+                                          float (*dst)[kPitch]) {
+  const int tid = threadIdx.x;
+  for (int e = tid; e < kTile * kDepth; e += 256) {
+    const int r = s_k == 1 ? e / kDepth : e % kTile;
+    const int c = s_k == 1 ? e % kDepth : e / kTile;
+    dst[r][c] =
+        r < rows && c < depth ? to_f(src[r * s_row + c * s_k]) : 0.f;
+  }
+}
+
+__device__ __forceinline__ void tile_products(const float (*a)[kPitch],
+                                              const float (*b)[kPitch],
+                                              f32x4 (&acc)[2][2]) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int r = lane & 15, q = lane >> 4;
+  const int m0 = (wave >> 1) * 32, n0 = (wave & 1) * 32;
+#pragma unroll
+  for (int c = 0; c < kDepth; c += 16) {
+    f32x4 av[2], bv[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      av[i] = *reinterpret_cast<const f32x4*>(&a[m0 + i * 16 + r][c + q * 4]);
+      bv[i] = *reinterpret_cast<const f32x4*>(&b[n0 + i * 16 + r][c + q * 4]);
+    }
+#pragma unroll
+    for (int s = 0; s < 4; ++s)
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+          acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(
+              av[i][s], bv[j][s], acc[i][j], 0, 0, 0);
+  }
+}
+
+// out[s, n] = sum_c a[s, c] * w[g(s)][n * s_n + c * s_c] (+ bias[g(s), n])
+template <typename T>
+__global__ __launch_bounds__(256) void product_plain_kernel(
+    const T* __restrict__ a, long a_pitch, const T* __restrict__ w,
+    long w_group, long s_n, long s_c, const T* __restrict__ bias,
+    const int* __restrict__ offsets, int G, int M, int N, int C,
+    T* __restrict__ out) {
+  const Segment seg = find_segment<kTile>(offsets, G, M, blockIdx.x);
+  if (seg.first >= seg.end) return;
+  __shared__ __align__(16) float As[kTile][kPitch], Bs[kTile][kPitch];
+  const int rows = min(kTile, seg.end - seg.first);
+  const int n0 = blockIdx.y * kTile;
+  const int cols = min(kTile, N - n0);
+  f32x4 acc[2][2] = {};
+  if (seg.group < G) {
+    const T* ga = a + seg.first * a_pitch;
+    const T* gw = w + seg.group * w_group + n0 * s_n;
+    for (int c = 0; c < C; c += kDepth) {
+      __syncthreads();
+      load_tile(ga + c, a_pitch, 1, rows, C - c, As);
+      load_tile(gw + c * s_c, s_n, s_c, cols, C - c, Bs);
+      __syncthreads();
+      tile_products(As, Bs, acc);
+    }
+  }
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int m = (wave >> 1) * 32 + i * 16 + (lane >> 4) * 4 + r;
+        const int n = (wave & 1) * 32 + j * 16 + (lane & 15);
+        if (m >= rows || n >= cols) continue;
+        float v = acc[i][j][r];
+        if (bias && seg.group < G)
+          v += to_f(bias[(long)seg.group * N + n0 + n]);
+        out[(long)(seg.first + m) * N + n0 + n] = (T)v;
+      }
+}
+
+// dw[g, n, f] = sum over the group's rows of dy[s, n] * x[s, f]; the blocks
+// of the first column tile sum db[g, n] too.
+template <typename T>
+__global__ __launch_bounds__(256) void weights_plain_kernel(
+    const T* __restrict__ dy, long dy_pitch, const T* __restrict__ x,
+    long x_pitch, const int* __restrict__ offsets, int G, int M, int N, int F,
+    T* __restrict__ dw, T* __restrict__ db) {
+  __shared__ __align__(16) float As[kTile][kPitch], Bs[kTile][kPitch];
+  const int g = blockIdx.x;
+  const int n0 = blockIdx.y * kTile;
+  const int f0 = blockIdx.z * kTile;
+  const int first = edge(offsets, g, G, M), end = edge(offsets, g + 1, G, M);
+  const int ns = min(kTile, N - n0), fs = min(kTile, F - f0);
+  f32x4 acc[2][2] = {};
+  float sum = 0.f;
+  for (int s = first; s < end; s += kDepth) {
+    __syncthreads();
+    load_tile(dy + (long)s * dy_pitch + n0, 1, dy_pitch, ns, end - s, As);
+    load_tile(x + (long)s * x_pitch + f0, 1, x_pitch, fs, end - s, Bs);
+    __syncthreads();
+    tile_products(As, Bs, acc);
+    if (threadIdx.x < kTile)
+      for (int c = 0; c < kDepth; ++c) sum += As[threadIdx.x][c];
+  }
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int n = (wave >> 1) * 32 + i * 16 + (lane >> 4) * 4 + r;
+        const int f = (wave & 1) * 32 + j * 16 + (lane & 15);
+        if (n < ns && f < fs)
+          dw[((long)g * N + n0 + n) * F + f0 + f] = (T)acc[i][j][r];
+      }
+  if (db && blockIdx.z == 0 && threadIdx.x < ns)
+    db[(long)g * N + n0 + threadIdx.x] = (T)sum;
+}
+
+void check_product(const at::Tensor& a, const at::Tensor& weight,
+                   const at::Tensor& offsets) {
+  TORCH_CHECK(a.is_cuda() && a.dim() == 2, "rows must be a GPU matrix");
+  TORCH_CHECK(weight.dim() == 3 && weight.dtype() == a.dtype() &&
+                  weight.device() == a.device() && weight.is_contiguous(),
+              "weight must be contiguous [G, N, F] of the rows' type");
+  TORCH_CHECK(offsets.dtype() == at::kInt && offsets.dim() == 1 &&
+                  offsets.numel() == weight.size(0) + 1 &&
+                  offsets.is_contiguous() && offsets.device() == a.device(),
+              "offsets must be contiguous int32 [G + 1]");
+  TORCH_CHECK(weight.size(0) >= 1 && weight.size(0) < (1 << 24),
+              "between 1 and 2^24 - 1 groups");
+  TORCH_CHECK(a.size(0) < (1ll << 31) - 65536 &&
+                  weight.size(1) < (1 << 21) && weight.size(2) < (1 << 21),
+              "too many rows, or rows that are too wide");
+}
+
+at::Tensor product(const at::Tensor& a_in, const at::Tensor& weight,
+                   const at::Tensor& offsets,
+                   const c10::optional<at::Tensor>& bias, bool transposed) {
+  check_product(a_in, weight, offsets);
+  const int G = (int)weight.size(0);
+  const int N = (int)weight.size(transposed ? 2 : 1);
+  const int C = (int)weight.size(transposed ? 1 : 2);
+  TORCH_CHECK(a_in.size(1) == C, "rows and weights differ in width");
+  if (bias)
+    TORCH_CHECK(bias->dim() == 2 && bias->size(0) == G &&
+                    bias->size(1) == N && bias->is_contiguous() &&
+                    bias->dtype() == a_in.dtype() &&
+                    bias->device() == a_in.device(),
+                "bias must be contiguous [G, N] of the rows' type");
+  c10::cuda::CUDAGuard guard(a_in.device());
+  at::Tensor a = packed_rows(a_in);
+  const int M = (int)a.size(0);
+  at::Tensor out = at::empty({M, N}, a.options());
+  if (out.numel() == 0) return out;
+  SKA_TYPES(a.scalar_type(), [&] {
+    dim3 grid(M / kTile + G + 1, (N + kTile - 1) / kTile);
+    TORCH_CHECK(grid.y < 65536, "rows are too wide");
+    product_plain_kernel<T><<<grid, 256, 0, stream_now()>>>(
+        ptr<T>(a), a.stride(0), ptr<T>(weight), (long)N * C,
+        transposed ? 1 : C, transposed ? N : 1,
+        bias ? ptr<T>(*bias) : nullptr, offsets.data_ptr<int>(), G, M, N, C,
+        ptr<T>(out));
+    check_launch();
+  });
+  return out;
+}
+
+at::Tensor grouped_linear(const at::Tensor& rows, const at::Tensor& weight,
+                          const at::Tensor& offsets,
+                          const c10::optional<at::Tensor>& bias) {
+  return product(rows, weight, offsets, bias, false);
+}
+
+at::Tensor grouped_linear_drows(const at::Tensor& dy,
+                                const at::Tensor& weight,
+                                const at::Tensor& offsets) {
+  return product(dy, weight, offsets, c10::nullopt, true);
+}
+
+std::tuple<at::Tensor, c10::optional<at::Tensor>> grouped_linear_dweight(
+    const at::Tensor& dy_in, const at::Tensor& rows_in,
+    const at::Tensor& offsets, bool need_bias) {
+  TORCH_CHECK(dy_in.is_cuda() && dy_in.dim() == 2 && rows_in.dim() == 2 &&
+                  rows_in.device() == dy_in.device() &&
+                  rows_in.dtype() == dy_in.dtype() &&
+                  rows_in.size(0) == dy_in.size(0),
+              "dy and rows must be GPU matrices of one type and length");
+  TORCH_CHECK(offsets.dtype() == at::kInt && offsets.dim() == 1 &&
+                  offsets.numel() >= 2 && offsets.numel() <= (1 << 24) &&
+                  offsets.is_contiguous() &&
+                  offsets.device() == dy_in.device(),
+              "offsets must be contiguous int32 [G + 1]");
+  TORCH_CHECK(dy_in.size(0) < (1ll << 31) - 65536 &&
+                  dy_in.size(1) < (1 << 21) && rows_in.size(1) < (1 << 21),
+              "too many rows, or rows that are too wide");
+  c10::cuda::CUDAGuard guard(dy_in.device());
+  at::Tensor dy = packed_rows(dy_in), x = packed_rows(rows_in);
+  const int G = (int)offsets.numel() - 1, M = (int)dy.size(0);
+  const int N = (int)dy.size(1), F = (int)x.size(1);
+  at::Tensor dw = at::empty({G, N, F}, dy.options());
+  c10::optional<at::Tensor> db;
+  if (need_bias) db = at::empty({G, N}, dy.options());
+  if (N == 0) return {dw, db};
+  SKA_TYPES(dy.scalar_type(), [&] {
+    // at least one column tile, which sums the bias where F is 0
+    dim3 grid(G, (N + kTile - 1) / kTile, std::max(1, (F + kTile - 1) / kTile));
+    TORCH_CHECK(grid.y < 65536 && grid.z < 65536, "rows are too wide");
+    weights_plain_kernel<T><<<grid, 256, 0, stream_now()>>>(
+        ptr<T>(dy), dy.stride(0), ptr<T>(x), x.stride(0),
+        offsets.data_ptr<int>(), G, M, N, F, ptr<T>(dw),
+        db ? ptr<T>(*db) : nullptr);
+    check_launch();
+  });
+  return {dw, db};
+}
+
+}  // namespace
+
+void bind_grouped(pybind11::module_& m) {
+  m.def("group_rows", &group_rows, "stable sort of rows by group");
+  m.def("gather_rows", &gather_rows, "rows into group order");
+  m.def("combine_rows", &combine_rows, "weighted rows back into row order");
+  m.def("combine_rows_backward", &combine_rows_backward);
+  m.def("grouped_linear", &grouped_linear,
+        "each group's rows times its weights");
+  m.def("grouped_linear_drows", &grouped_linear_drows);
+  m.def("grouped_linear_dweight", &grouped_linear_dweight);
+}

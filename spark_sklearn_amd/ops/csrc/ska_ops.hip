@@ -7187,7 +7187,10 @@ std::vector<double> flagship_ablate(int64_t rows, int64_t Fp, int64_t iters) {
   return out;
 }
 
+void bind_grouped(pybind11::module_& m);  // ska_grouped.hip
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
+  bind_grouped(m);
   m.def("flagship_ablate", &flagship_ablate,
         "ablation timings for the fwd kernel (ms/launch)");
   m.def("gemm_probe", &gemm_probe, "MFMA layout probe (4 combos)");
