@@ -83,11 +83,20 @@ class KeyedEstimator:
     ``estimatorType`` in {"predictor", "transformer", "clusterer"}
     (inferred when omitted: yCol given -> predictor; estimator has
     ``predict`` but no y -> clusterer; else transformer).
+
+    ``keySolver`` says how the linear family of
+    :mod:`spark_sklearn_amd.models` is fitted.  "columns": on a GPU, keys are
+    columns of a launch that reads the rows of all keys for each (bfloat16
+    matrix).  "grouped": rows are sorted by key and each key's rows meet that
+    key's weights alone (float32 matrix), on the GPU or on the CPU; the form
+    for many keys.  Both leave other estimators, sparse rows, ``class_weight``
+    and keys that lack some of the classes to the host, one key at a time.
     """
 
     def __init__(self, sklearnEstimator=None, keyCols: Optional[List[str]] = None,
                  xCol: str = "features", yCol: Optional[str] = None,
-                 estimatorType: Optional[str] = None):
+                 estimatorType: Optional[str] = None,
+                 keySolver: str = "columns"):
         if sklearnEstimator is None:
             raise ValueError("sklearnEstimator must be provided")
         if not (hasattr(sklearnEstimator, "fit") and
@@ -111,6 +120,11 @@ class KeyedEstimator:
         if estimatorType == "predictor" and yCol is None:
             raise ValueError("estimatorType='predictor' requires yCol")
         self.estimatorType = estimatorType
+        if keySolver not in ("columns", "grouped"):
+            raise ValueError(
+                f"keySolver must be 'columns' or 'grouped', got "
+                f"{keySolver!r}")
+        self.keySolver = keySolver
 
     def fit(self, df: pd.DataFrame) -> "KeyedModel":
         missing = [c for c in self.keyCols + [self.xCol] if c not in df.columns]
@@ -121,7 +135,10 @@ class KeyedEstimator:
 
         groups = [((key if isinstance(key, tuple) else (key,)), group)
                   for key, group in df.groupby(self.keyCols, sort=True)]
-        fitted = self._fit_keys_batched(groups)
+        if self.keySolver == "grouped":
+            fitted = self._fit_keys_grouped(groups)
+        else:
+            fitted = self._fit_keys_batched(groups)
         if fitted is None:
             fitted = []
             for key, group in groups:
@@ -237,6 +254,49 @@ class KeyedEstimator:
         return fitted
 
 
+    def _fit_keys_grouped(self, groups):
+        """All keys of the linear family at once through the grouped-row
+        operators (``ops/keyed_executor.py``).  Returns None when the keys
+        have to be fitted one at a time."""
+        proto = self.sklearnEstimator
+        if getattr(type(proto), "_engine_family", None) != "linear" or \
+                self.yCol is None or not groups or \
+                getattr(proto, "class_weight", None) is not None:
+            return None
+        from sklearn.base import is_classifier
+
+        ys = [np.asarray(g[self.yCol].values) for _, g in groups]
+        Xs = [_stack_feature_column(g[self.xCol].values) for _, g in groups]
+        if any(not isinstance(x, np.ndarray) for x in Xs) or \
+                len({x.shape[1] for x in Xs}) != 1:
+            return None
+        classes, n_classes = None, 0
+        y_all = np.concatenate(ys)
+        if is_classifier(proto):
+            classes, y_all = np.unique(y_all, return_inverse=True)
+            n_classes = len(classes)
+            if n_classes < 2 or \
+                    any(len(np.unique(y)) != n_classes for y in ys):
+                return None
+        from .engine import _device_or_none
+        from .ops.keyed_executor import KeyedLinearExecutor
+
+        row_key = np.repeat(np.arange(len(groups)), [len(x) for x in Xs])
+        executor = KeyedLinearExecutor(
+            np.concatenate(Xs), y_all, row_key, len(groups),
+            _device_or_none(None))
+        specs = [proto._column_spec(int(n), float(m))
+                 for n, m in zip(executor.counts, executor.msq)]
+        W, b, n_iter = executor.fit(specs, n_classes)
+        fitted = []
+        for slot, (key, _) in enumerate(groups):
+            est = clone(proto)
+            est._finalize_fit(np.ascontiguousarray(W[slot].T), b[slot],
+                              n_iter[slot], classes)
+            fitted.append(tuple(key) + (SparkSklearnEstimator(est),))
+        return fitted
+
+
 class KeyedModel:
     """The fitted per-key model table; ``transform`` applies per-row.
 
@@ -258,10 +318,19 @@ class KeyedModel:
     def outputCol(self) -> str:
         return "output" if self.estimatorType == "transformer" else "prediction"
 
-    def transform(self, df: pd.DataFrame,
-                  unseenKeys: str = "error") -> pd.DataFrame:
+    def transform(self, df: pd.DataFrame, unseenKeys: str = "error",
+                  device=None) -> pd.DataFrame:
+        """Append each row's result.
+
+        ``device`` ("cuda", "cpu" or a torch.device): score all keys' rows
+        together there, in float32, by the grouped-row operators.  For models
+        of the linear family in :mod:`spark_sklearn_amd.models` and dense
+        rows.  None: one key at a time on the host, in float64.
+        """
         if unseenKeys not in ("error", "drop"):
             raise ValueError("unseenKeys must be 'error' or 'drop'")
+        if device is not None:
+            return self._transform_grouped(df, unseenKeys, device)
         model_map = {
             tuple(row[c] for c in self.keyCols): row["estimator"].estimator
             for _, row in self.keyedModels.iterrows()
@@ -291,3 +360,68 @@ class KeyedModel:
             empty[self.outputCol] = []
             return empty
         return pd.concat(out_frames).sort_index()
+
+    def _transform_grouped(self, df, unseenKeys, device):
+        models = self.keyedModels.drop_duplicates(self.keyCols, keep="last")
+        ests = [e.estimator for e in models["estimator"]]
+        if self.estimatorType != "predictor" or not ests or any(
+                getattr(type(e), "_engine_family", None) != "linear"
+                for e in ests):
+            raise ValueError(
+                "device= scores fitted predictors of the linear family; "
+                "use device=None for others")
+        if df[self.keyCols].isna().any(axis=1).any():
+            # grouping by key passes over rows without one
+            df = df[df[self.keyCols].notna().all(axis=1)]
+
+        def index(frame):
+            if len(self.keyCols) == 1:
+                return pd.Index(frame[self.keyCols[0]])
+            return pd.MultiIndex.from_frame(frame[self.keyCols])
+
+        row_key = index(models).get_indexer(index(df))
+        if (row_key < 0).any():
+            if unseenKeys == "error":
+                first = df.iloc[int(np.argmax(row_key < 0))]
+                key = tuple(first[c] for c in self.keyCols)
+                raise KeyError(
+                    f"no fitted model for key {key!r}; fit() never saw it")
+            df, row_key = df[row_key >= 0], row_key[row_key >= 0]
+        if len(df) == 0:
+            empty = df.copy()
+            empty[self.outputCol] = []
+            return empty
+        X = _stack_feature_column(df[self.xCol].values)
+        if not isinstance(X, np.ndarray):
+            raise ValueError("device= takes dense rows")
+        coefs = [np.atleast_2d(e.coef_) for e in ests]
+        if {c.shape[1] for c in coefs} != {X.shape[1]}:
+            raise ValueError(
+                f"rows have {X.shape[1]} features, the models "
+                f"{sorted({c.shape[1] for c in coefs})}")
+        widths = np.array([len(c) for c in coefs])
+        C = int(widths.max())
+        coef = np.zeros((len(ests), C, X.shape[1]), np.float32)
+        # a class that a key's model does not have is never the largest
+        intercept = np.full((len(ests), C), -np.inf, np.float32)
+        for g, (e, c) in enumerate(zip(ests, coefs)):
+            coef[g, :len(c)] = c
+            intercept[g, :len(c)] = np.atleast_1d(e.intercept_)
+        import torch
+
+        from .ops.keyed_executor import keyed_scores
+
+        scores = keyed_scores(X, row_key, coef, intercept,
+                              torch.device(device))
+        out = df.copy()
+        if hasattr(ests[0], "classes_"):
+            best = np.where(widths[row_key] == 1, scores[:, 0] > 0,
+                            np.argmax(scores, axis=1))
+            labels = np.empty((len(ests), int(best.max()) + 1), object)
+            for g, e in enumerate(ests):
+                known = list(e.classes_[:labels.shape[1]])
+                labels[g, :len(known)] = known
+            out[self.outputCol] = list(labels[row_key, best])
+        else:
+            out[self.outputCol] = scores[:, 0].astype(np.float64)
+        return out.sort_index()
