@@ -648,21 +648,30 @@ __device__ __forceinline__ int edge(const int* offsets, int g, int G, int M) {
   return g <= 0 ? 0 : (g > G ? M : clampi(offsets[g], 0, M));
 }
 
+// The last group whose first tile is not behind `tile`: each round, 64 lanes
+// look at 64 evenly spaced groups, so that 4095 groups take two reads.
 template <int BM>
 __device__ __forceinline__ Segment find_segment(const int* offsets, int G,
                                                 int M, int tile) {
-  int lo = 0, hi = G + 1;  // the last group whose first tile is not behind
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (edge(offsets, mid, G, M) / BM + mid <= tile)
-      lo = mid;
-    else
-      hi = mid;
+  const int lane = threadIdx.x & 63;
+  int lo = 0, n = G + 1;
+  while (n > 1) {
+    const int step = (n + 63) >> 6;
+    const int g = lo + lane * step;
+    const bool at = lane * step < n && edge(offsets, g, G, M) / BM + g <= tile;
+    // offsets do not decrease, so these are the lanes up to some lane; lane 0
+    // counts in any case
+    const unsigned long long set = __ballot(at) | 1ull;
+    const int last = 63 - __builtin_clzll(set);
+    lo += last * step;
+    n = min(step, n - last * step);
   }
+  lo = __builtin_amdgcn_readfirstlane(lo);
   const int start = edge(offsets, lo, G, M);
   const int end = edge(offsets, lo + 1, G, M);
   const long first = start + (long)(tile - (start / BM + lo)) * BM;
-  return {lo, (int)min(first, (long)end), end};
+  return {lo, __builtin_amdgcn_readfirstlane((int)min(first, (long)end)),
+          __builtin_amdgcn_readfirstlane(end)};
 }
 
 // The plain tile: 64 x 64 outputs, 32 steps of the contraction at a time in
@@ -789,6 +798,367 @@ __global__ __launch_bounds__(256) void weights_plain_kernel(
     db[(long)g * N + n0 + threadIdx.x] = (T)sum;
 }
 
+
+// ---------------------------------------------------------------------------
+// 16-bit products on v_mfma_f32_16x16x32.  All three are
+//
+//     out[m, n] = sum_c A[m, c] * B[n, c]
+//
+//   forward   A = rows (m = s, c = f)    B = weight[g] (n, c = f)
+//   drows     A = dy   (m = s, c = n')   B = weight[g] (n = f, c = n')
+//   dweight   A = dy   (m = n', c = s)   B = rows      (n = f, c = s)
+//
+// An operand lies in memory along c ("along") or across it ("across": m or n
+// is the contiguous index).  Tiles of 64 steps of c go to LDS in granules of
+// 8 values, by buffer loads that write LDS themselves; a lane out of range
+// writes zeros.  An along tile is [m][64]: granule j of row m lies at
+// j ^ (m & 7), and a fragment is one 16-byte read.  An across tile is
+// [64][m]: its fragments are two transposing reads of 4 values of c each
+// (16 lanes read 4 rows of 32 bytes), and granules are moved by bits of c so
+// that these rows lie in different banks.
+//
+// The matrix instruction gets B first: a lane then holds 4 neighbouring n of
+// one m, and stores them together.
+// ---------------------------------------------------------------------------
+constexpr int kStep = 64;
+enum Mode { kForward, kDRows, kDWeight };
+
+template <typename T>
+struct Mma;
+template <>
+struct Mma<__bf16> {
+  typedef __bf16 Frag __attribute__((ext_vector_type(8)));
+  static __device__ __forceinline__ f32x4 go(Frag a, Frag b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+  }
+};
+template <>
+struct Mma<_Float16> {
+  typedef _Float16 Frag __attribute__((ext_vector_type(8)));
+  static __device__ __forceinline__ f32x4 go(Frag a, Frag b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+  }
+};
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+#define SKA_LDS(T, p) ((__attribute__((address_space(3))) T*)(p))
+
+// One operand's tile of EXT rows (m or n) by kStep steps of c.
+template <typename T, int EXT, bool ACROSS, int THREADS>
+struct Tile {
+  static constexpr int kGranules = EXT * kStep / 8;
+  static constexpr int kPer = kGranules / THREADS;
+  static constexpr int kAcross = EXT / 8;  // granules of one step of c
+  static constexpr int kBytes = EXT * kStep * 2;
+
+  static __device__ __forceinline__ int move(int c) {
+    return (((c & 3) << 1) | (((c >> 3) & 1) << 3)) & (kAcross - 1);
+  }
+  // the first row and step of the granule at LDS place g
+  static __device__ __forceinline__ void place(int g, int& row, int& c) {
+    if (ACROSS) {
+      c = g / kAcross;
+      row = ((g % kAcross) ^ move(c)) * 8;
+    } else {
+      row = g >> 3;
+      c = ((g & 7) ^ (row & 7)) * 8;
+    }
+  }
+  // Which part of a granule may be read: 8 for all of it.  `room` is the
+  // number of values from `src` to the end of the matrix: an across granule
+  // may run into the next row, whose values meet outputs that are not stored.
+  static __device__ __forceinline__ int part(int row, int c, long pitch,
+                                             int rows, int steps, long room) {
+    if (row >= rows || c >= steps) return 0;
+    if (ACROSS) {
+      const int n = rows - row;
+      return n >= 8 || c * pitch + row + 8 <= room ? 8 : n;
+    }
+    return min(8, steps - c);
+  }
+  static __device__ __forceinline__ long at(int row, int c, long pitch) {
+    return ACROSS ? c * pitch + row : row * pitch + c;
+  }
+  // whether any granule is read in part
+  static __device__ __forceinline__ bool ragged(long pitch, int rows,
+                                                int steps, long room) {
+    if (ACROSS)
+      return (rows & 7) &&
+             (min(steps, kStep) - 1) * pitch + ((rows + 7) & ~7) > room;
+    return steps < kStep && (steps & 7);
+  }
+  static __device__ __forceinline__ void load_async(const T* src, long pitch,
+                                                    int rows, int steps,
+                                                    long room, char* lds) {
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(
+        (void*)src, 0, 0x7fffffff, 0x00020000);
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int g0 = i * THREADS + wave * 64;
+      int row, c;
+      place(g0 + lane, row, c);
+      const bool in = part(row, c, pitch, rows, steps, room) == 8;
+      const unsigned off = in ? (unsigned)at(row, c, pitch) * 2 : 0x80000000u;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(
+          rsrc, SKA_LDS(void, lds + g0 * 16), 16, off, 0, 0, 0);
+    }
+  }
+  // after the loads above have ended: the granules that were left out
+  static __device__ __forceinline__ void fill(const T* src, long pitch,
+                                              int rows, int steps, long room,
+                                              char* lds) {
+#pragma unroll 1
+    for (int i = 0; i < kPer; ++i) {
+      const int g = i * THREADS + threadIdx.x;
+      int row, c;
+      place(g, row, c);
+      const int n = part(row, c, pitch, rows, steps, room);
+      if (n == 0 || n == 8) continue;
+      T* to = reinterpret_cast<T*>(lds + g * 16);
+      const T* from = src + at(row, c, pitch);
+      for (int e = 0; e < n; ++e) to[e] = from[e];
+    }
+  }
+  // rows that begin at odd addresses: through registers
+  static __device__ __forceinline__ void load_regs(const T* src, long pitch,
+                                                   int rows, int steps,
+                                                   long room,
+                                                   Vec<T> (&v)[kPer]) {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      int row, c;
+      place(i * THREADS + threadIdx.x, row, c);
+      const int n = part(row, c, pitch, rows, steps, room);
+      v[i] = load_vec(src + (n ? at(row, c, pitch) : 0), n);
+    }
+  }
+  static __device__ __forceinline__ void store_regs(const Vec<T> (&v)[kPer],
+                                                    char* lds) {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+      *reinterpret_cast<Vec<T>*>(lds + (i * THREADS + threadIdx.x) * 16) =
+          v[i];
+  }
+  // the fragment of rows [row0, row0 + 16) and steps [c0, c0 + 32)
+  static __device__ __forceinline__ typename Mma<T>::Frag frag(
+      const char* lds, int row0, int c0) {
+    const int lane = threadIdx.x & 63;
+    const int r = lane & 15, q = lane >> 4;
+    if (ACROSS) {
+      s16x4 v[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int c = c0 + q * 8 + h * 4 + (r >> 2);
+        const int g = ((row0 >> 3) + ((r & 3) >> 1)) ^ move(c);
+        v[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            SKA_LDS(s16x4, lds + (c * kAcross + g) * 16 + (r & 1) * 8));
+      }
+      const s16x8 w = {v[0][0], v[0][1], v[0][2], v[0][3],
+                       v[1][0], v[1][1], v[1][2], v[1][3]};
+      return __builtin_bit_cast(typename Mma<T>::Frag, w);
+    }
+    const int row = row0 + r;
+    return *reinterpret_cast<const typename Mma<T>::Frag*>(
+        lds + (row * 8 + (((c0 >> 3) + q) ^ (row & 7))) * 16);
+  }
+};
+
+struct Product {
+  const void* a;
+  const void* b;
+  const void* bias;  // forward: [G, N]
+  void* out;
+  void* sums;  // dweight: the sum of A over c, [G, N]
+  const int* offsets;
+  long a_pitch, b_pitch;
+  int G, M, N, C;  // dweight: M rows of out a group, C rows in all
+};
+
+template <typename T, int BM, int BN, int WM, int WN, int MODE, bool ASYNC>
+__global__ __launch_bounds__(WM* WN * 64) void product_kernel(Product p) {
+  constexpr int kThreads = WM * WN * 64;
+  constexpr int FM = BM / WM / 16, FN = BN / WN / 16;
+  typedef Tile<T, BM, MODE == kDWeight, kThreads> TA;
+  typedef Tile<T, BN, MODE != kForward, kThreads> TB;
+  __shared__ __align__(16) char lds[2][TA::kBytes + TB::kBytes];
+
+  // Blocks go round the 8 XCDs: each gets a contiguous run of tiles, whose
+  // operands its L2 then holds.
+  const int each = gridDim.x >> 3;
+  int tile = blockIdx.x;
+  if (tile < each * 8) tile = (tile & 7) * each + (tile >> 3);
+  const int nt = (p.N + BN - 1) / BN;
+  const int n0 = (tile % nt) * BN;
+  tile /= nt;
+
+  const T* A = reinterpret_cast<const T*>(p.a);
+  const T* B = reinterpret_cast<const T*>(p.b);
+  int group, rows, steps;  // of out; steps of c
+  long out_row, a_room, b_room;
+  if (MODE == kDWeight) {
+    const int mt = (p.M + BM - 1) / BM;
+    group = tile / mt;
+    const int m0 = (tile % mt) * BM;
+    const int first = edge(p.offsets, group, p.G, p.C);
+    steps = edge(p.offsets, group + 1, p.G, p.C) - first;
+    rows = min(BM, p.M - m0);
+    out_row = (long)group * p.M + m0;
+    A += first * p.a_pitch + m0;
+    B += first * p.b_pitch + n0;
+    a_room = (long)(p.C - first - 1) * p.a_pitch + p.M - m0;
+    b_room = (long)(p.C - first - 1) * p.b_pitch + p.N - n0;
+  } else {
+    const Segment seg = find_segment<BM>(p.offsets, p.G, p.M, tile);
+    if (seg.first >= seg.end) return;
+    group = seg.group;
+    rows = min(BM, seg.end - seg.first);
+    steps = group < p.G ? p.C : 0;
+    out_row = seg.first;
+    A += seg.first * p.a_pitch;
+    a_room = 0;
+    const long weights = (long)p.N * p.C;
+    B += min(group, p.G - 1) * weights +
+         (MODE == kForward ? n0 * (long)p.C : n0);
+    b_room = (long)(p.C - 1) * p.N + p.N - n0;
+    if (group < p.G - 1) b_room += weights;
+  }
+  const int cols = min(BN, p.N - n0);
+  const long a_step = MODE == kDWeight ? kStep * p.a_pitch : kStep;
+  const long b_step = MODE == kForward ? kStep : kStep * p.b_pitch;
+
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
+  const int wm = (wave / WN) * (BM / WM), wn = (wave % WN) * (BN / WN);
+  f32x4 acc[FM][FN] = {};
+  f32x4 sum[FM] = {};
+  const bool sums = MODE == kDWeight && p.sums && n0 == 0 && wave % WN == 0;
+  typename Mma<T>::Frag ones;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) ones[i] = (T)1.f;
+
+  Vec<T> ra[ASYNC ? 1 : TA::kPer], rb[ASYNC ? 1 : TB::kPer];
+  auto load = [&](int c, int buf) {
+    const long left = (long)(c / kStep);
+    const T* a = A + left * a_step;
+    const T* b = B + left * b_step;
+    if constexpr (ASYNC) {
+      TA::load_async(a, p.a_pitch, rows, steps - c, a_room - left * a_step,
+                     lds[buf]);
+      TB::load_async(b, p.b_pitch, cols, steps - c, b_room - left * b_step,
+                     lds[buf] + TA::kBytes);
+    } else {
+      TA::load_regs(a, p.a_pitch, rows, steps - c, a_room - left * a_step,
+                    ra);
+      TB::load_regs(b, p.b_pitch, cols, steps - c, b_room - left * b_step,
+                    rb);
+    }
+  };
+  auto land = [&](int c, int buf) {
+    if constexpr (ASYNC) {
+      __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
+      const long left = (long)(c / kStep);
+      const long ar = a_room - left * a_step, br = b_room - left * b_step;
+      if (TA::ragged(p.a_pitch, rows, steps - c, ar))
+        TA::fill(A + left * a_step, p.a_pitch, rows, steps - c, ar, lds[buf]);
+      if (TB::ragged(p.b_pitch, cols, steps - c, br))
+        TB::fill(B + left * b_step, p.b_pitch, cols, steps - c, br,
+                 lds[buf] + TA::kBytes);
+    } else {
+      TA::store_regs(ra, lds[buf]);
+      TB::store_regs(rb, lds[buf] + TA::kBytes);
+    }
+  };
+
+  if (steps > 0) load(0, 0);
+  for (int c = 0, buf = 0; c < steps; c += kStep, buf ^= 1) {
+    land(c, buf);
+    __syncthreads();
+    if (c + kStep < steps) load(c + kStep, buf ^ 1);
+    const char* la = lds[buf];
+    const char* lb = lds[buf] + TA::kBytes;
+#pragma unroll
+    for (int h = 0; h < kStep; h += 32) {
+      typename Mma<T>::Frag fb[FN];
+#pragma unroll
+      for (int j = 0; j < FN; ++j) fb[j] = TB::frag(lb, wn + j * 16, h);
+#pragma unroll
+      for (int i = 0; i < FM; ++i) {
+        const typename Mma<T>::Frag fa = TA::frag(la, wm + i * 16, h);
+#pragma unroll
+        for (int j = 0; j < FN; ++j)
+          acc[i][j] = Mma<T>::go(fb[j], fa, acc[i][j]);
+        if (MODE == kDWeight && sums) sum[i] = Mma<T>::go(ones, fa, sum[i]);
+      }
+    }
+  }
+
+  // lane: row m = lane & 15 of its tile, 4 columns from (lane >> 4) * 4
+  T* out = reinterpret_cast<T*>(p.out);
+  const T* bias = reinterpret_cast<const T*>(p.bias);
+#pragma unroll
+  for (int j = 0; j < FN; ++j) {
+    const int n = wn + j * 16 + (lane >> 4) * 4;
+    if (n >= cols) continue;
+    const int left = cols - n;
+    float add[4] = {};
+    if (MODE == kForward && bias && group < p.G) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (r < left) add[r] = to_f(bias[(long)group * p.N + n0 + n + r]);
+    }
+#pragma unroll
+    for (int i = 0; i < FM; ++i) {
+      const int m = wm + i * 16 + (lane & 15);
+      if (m >= rows) continue;
+      T v[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) v[r] = (T)(acc[i][j][r] + add[r]);
+      T* to = out + (out_row + m) * p.N + n0 + n;
+      if (left >= 4) {
+        __builtin_memcpy(to, v, 8);
+      } else {
+        for (int r = 0; r < left; ++r) to[r] = v[r];
+      }
+    }
+  }
+  if (sums && lane < 16) {
+#pragma unroll
+    for (int i = 0; i < FM; ++i) {
+      const int m = wm + i * 16 + lane;
+      if (m < rows) reinterpret_cast<T*>(p.sums)[out_row + m] = (T)sum[i][0];
+    }
+  }
+}
+
+// Buffer loads to LDS take addresses of whole words.
+template <typename T>
+bool whole_words(const T* p, long pitch) {
+  return (reinterpret_cast<uintptr_t>(p) & 3) == 0 && (pitch & 1) == 0;
+}
+
+template <typename T, int MODE>
+void product_launch(const Product& p) {
+  const bool async = whole_words((const T*)p.a, p.a_pitch) &&
+                     whole_words((const T*)p.b, p.b_pitch) &&
+                     // the weights of a group may begin at an odd value
+                     (MODE == kDWeight || ((long)p.N * p.C) % 2 == 0);
+  auto go = [&](auto kern, int bm, int bn, int threads) {
+    const long mt = MODE == kDWeight ? (long)p.G * ((p.M + bm - 1) / bm)
+                                     : (long)p.M / bm + p.G + 1;
+    const long blocks = mt * ((p.N + bn - 1) / bn);
+    TORCH_CHECK(blocks * threads < (1ll << 32), "too many tiles");
+    kern<<<(unsigned)blocks, threads, 0, stream_now()>>>(p);
+    check_launch();
+  };
+  if (async)
+    go(product_kernel<T, 256, 256, 2, 4, MODE, true>, 256, 256, 512);
+  else
+    go(product_kernel<T, 128, 128, 2, 2, MODE, false>, 128, 128, 256);
+}
+
 void check_product(const at::Tensor& a, const at::Tensor& weight,
                    const at::Tensor& offsets) {
   TORCH_CHECK(a.is_cuda() && a.dim() == 2, "rows must be a GPU matrix");
@@ -825,6 +1195,21 @@ at::Tensor product(const at::Tensor& a_in, const at::Tensor& weight,
   const int M = (int)a.size(0);
   at::Tensor out = at::empty({M, N}, a.options());
   if (out.numel() == 0) return out;
+  if (a.scalar_type() != at::kFloat) {
+    SKA_TYPES(a.scalar_type(), [&] {
+      if constexpr (sizeof(T) == 2) {
+        Product p{a.data_ptr(), weight.data_ptr(),
+                  bias ? bias->data_ptr() : nullptr, out.data_ptr(), nullptr,
+                  offsets.data_ptr<int>(), a.stride(0),
+                  transposed ? N : C, G, M, N, C};
+        if (transposed)
+          product_launch<T, kDRows>(p);
+        else
+          product_launch<T, kForward>(p);
+      }
+    });
+    return out;
+  }
   SKA_TYPES(a.scalar_type(), [&] {
     dim3 grid(M / kTile + G + 1, (N + kTile - 1) / kTile);
     TORCH_CHECK(grid.y < 65536, "rows are too wide");
@@ -874,6 +1259,16 @@ std::tuple<at::Tensor, c10::optional<at::Tensor>> grouped_linear_dweight(
   c10::optional<at::Tensor> db;
   if (need_bias) db = at::empty({G, N}, dy.options());
   if (N == 0) return {dw, db};
+  if (dy.scalar_type() != at::kFloat && F > 0 && M > 0) {
+    SKA_TYPES(dy.scalar_type(), [&] {
+      if constexpr (sizeof(T) == 2)
+        product_launch<T, kDWeight>(
+            Product{dy.data_ptr(), x.data_ptr(), nullptr, dw.data_ptr(),
+                    db ? db->data_ptr() : nullptr, offsets.data_ptr<int>(),
+                    dy.stride(0), x.stride(0), G, N, F, M});
+    });
+    return {dw, db};
+  }
   SKA_TYPES(dy.scalar_type(), [&] {
     // at least one column tile, which sums the bias where F is 0
     dim3 grid(G, (N + kTile - 1) / kTile, std::max(1, (F + kTile - 1) / kTile));
