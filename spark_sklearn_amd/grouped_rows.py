@@ -158,10 +158,10 @@ class _Reference:
         return grouped_linear_drows_ref(dy, weight, offsets)
 
     @staticmethod
-    def grouped_linear_dweight(dy, rows, offsets, need_bias):
+    def grouped_linear_dweight(*args):
         from .models._grouped_ref import grouped_linear_dweight_ref
 
-        return grouped_linear_dweight_ref(dy, rows, offsets, need_bias)
+        return grouped_linear_dweight_ref(*args)
 
 
 def _autograd():
@@ -224,13 +224,10 @@ def _autograd():
             drows = dweight = dbias = None
             if ctx.needs_input_grad[0]:
                 drows = k.grouped_linear_drows(grad, weight, offsets)
-            if ctx.needs_input_grad[1]:
+            if ctx.needs_input_grad[1] or ctx.needs_input_grad[3]:
                 dweight, dbias = k.grouped_linear_dweight(
-                    grad, rows, offsets, ctx.needs_input_grad[3])
-            elif ctx.needs_input_grad[3]:
-                # the bias alone: a product with rows of no width
-                _, dbias = k.grouped_linear_dweight(grad, rows[:, :0],
-                                                    offsets, True)
+                    grad, rows, offsets, ctx.needs_input_grad[1],
+                    ctx.needs_input_grad[3])
             return drows, dweight, None, dbias
 
     _functions = SimpleNamespace(Gather=Gather, Combine=Combine,

@@ -105,13 +105,15 @@ def grouped_linear_drows_ref(dy, weight, offsets):
     return out
 
 
-def grouped_linear_dweight_ref(dy, rows, offsets, need_bias):
+def grouped_linear_dweight_ref(dy, rows, offsets, need_weight, need_bias):
     G = offsets.numel() - 1
-    dw = torch.zeros(G, dy.shape[1], rows.shape[1], dtype=dy.dtype)
+    dw = torch.zeros(G, dy.shape[1], rows.shape[1],
+                     dtype=dy.dtype) if need_weight else None
     db = torch.zeros(G, dy.shape[1], dtype=dy.dtype) if need_bias else None
     for g, a, b in _runs(offsets):
         d = _wide(dy[a:b])
-        dw[g] = (d.t() @ _wide(rows[a:b])).to(dy.dtype)
+        if need_weight:
+            dw[g] = (d.t() @ _wide(rows[a:b])).to(dy.dtype)
         if need_bias:
             db[g] = d.sum(0).to(dy.dtype)
     return dw, db

@@ -633,45 +633,77 @@ combine_rows_backward(const at::Tensor& dy_in, const at::Tensor& rows_in,
 }
 
 // ---------------------------------------------------------------------------
-// Grouped products.  Row tiles are cut inside each group.  Tile i is found
-// from the offsets alone: group g's first tile has the index
-// floor(offsets[g] / BM) + g, which leaves every group room for its tiles
-// (ceil(n / BM) <= floor((a + n) / BM) - floor(a / BM) + 1), so the grid needs
+// Grouped products.  Row tiles (2^shift rows) are cut inside each group.  Tile
+// i is found from the offsets alone: group g's first tile has the index
+// floor(offsets[g] / 2^shift) + g, which leaves every group room for its tiles
+// (ceil(n / R) <= floor((a + n) / R) - floor(a / R) + 1), so the grid needs
 // no count from the device.  The rows behind the last group are a group of
 // their own, whose outputs are zero.
 // ---------------------------------------------------------------------------
 struct Segment {
-  int group, first, end;  // first >= end: nothing to do
+  int group, start, first, end;  // the tile's rows; first >= end: none
 };
 
 __device__ __forceinline__ int edge(const int* offsets, int g, int G, int M) {
   return g <= 0 ? 0 : (g > G ? M : clampi(offsets[g], 0, M));
 }
 
-// The last group whose first tile is not behind `tile`: each round, 64 lanes
-// look at 64 evenly spaced groups, so that 4095 groups take two reads.
-template <int BM>
-__device__ __forceinline__ Segment find_segment(const int* offsets, int G,
-                                                int M, int tile) {
+// The last group g with floor(offsets[g] >> shift) + g * each <= at.  Each
+// round, 64 lanes look at 64 evenly spaced groups: 4095 groups take two.
+__device__ __forceinline__ int find_group(const int* offsets, int G, int M,
+                                          int at, int shift, int each) {
   const int lane = threadIdx.x & 63;
   int lo = 0, n = G + 1;
   while (n > 1) {
     const int step = (n + 63) >> 6;
     const int g = lo + lane * step;
-    const bool at = lane * step < n && edge(offsets, g, G, M) / BM + g <= tile;
+    const bool in =
+        lane * step < n && (edge(offsets, g, G, M) >> shift) + g * each <= at;
     // offsets do not decrease, so these are the lanes up to some lane; lane 0
     // counts in any case
-    const unsigned long long set = __ballot(at) | 1ull;
+    const unsigned long long set = __ballot(in) | 1ull;
     const int last = 63 - __builtin_clzll(set);
     lo += last * step;
     n = min(step, n - last * step);
   }
-  lo = __builtin_amdgcn_readfirstlane(lo);
-  const int start = edge(offsets, lo, G, M);
-  const int end = edge(offsets, lo + 1, G, M);
-  const long first = start + (long)(tile - (start / BM + lo)) * BM;
-  return {lo, __builtin_amdgcn_readfirstlane((int)min(first, (long)end)),
+  return __builtin_amdgcn_readfirstlane(lo);
+}
+
+__device__ __forceinline__ Segment find_segment(const int* offsets, int G,
+                                                int M, int tile, int shift) {
+  const int g = find_group(offsets, G, M, tile, shift, 1);
+  const int start = edge(offsets, g, G, M);
+  const int end = edge(offsets, g + 1, G, M);
+  const long first =
+      start + ((long)(tile - ((start >> shift) + g)) << shift);
+  return {g, __builtin_amdgcn_readfirstlane(start),
+          __builtin_amdgcn_readfirstlane((int)min(first, (long)end)),
           __builtin_amdgcn_readfirstlane(end)};
+}
+
+// Where a part of a group's rows leaves its sums.  A group of n > R = 2^shift
+// rows has ceil(n / R) <= 2 floor(n / R) parts, so that the places of two such
+// groups do not meet and 2 (rows / R + 1) of them are enough.
+__device__ __forceinline__ long part_place(int start, int shift) {
+  return 2l * (start >> shift);
+}
+
+// Where there are more groups than rows: one block a row, which has the tile
+// that begins at its row, if one does.
+__device__ __forceinline__ Segment find_segment_at(const int* offsets, int G,
+                                                   int M, int row,
+                                                   int shift) {
+  const int g = find_group(offsets, G, M, row, 0, 0);
+  const int start = edge(offsets, g, G, M);
+  const int end = edge(offsets, g + 1, G, M);
+  const bool head = ((row - start) & ((1 << shift) - 1)) == 0;
+  return {g, __builtin_amdgcn_readfirstlane(start),
+          __builtin_amdgcn_readfirstlane(head ? row : end),
+          __builtin_amdgcn_readfirstlane(end)};
+}
+
+__host__ __device__ constexpr int log2_of(int v) {
+  return v <= 1 ? 0 : 1 + log2_of(v >> 1);
 }
 
 // The plain tile: 64 x 64 outputs, 32 steps of the contraction at a time in
@@ -723,7 +755,8 @@ __global__ __launch_bounds__(256) void product_plain_kernel(
     long w_group, long s_n, long s_c, const T* __restrict__ bias,
     const int* __restrict__ offsets, int G, int M, int N, int C,
     T* __restrict__ out) {
-  const Segment seg = find_segment<kTile>(offsets, G, M, blockIdx.x);
+  const Segment seg =
+      find_segment(offsets, G, M, blockIdx.x, log2_of(kTile));
   if (seg.first >= seg.end) return;
   __shared__ __align__(16) float As[kTile][kPitch], Bs[kTile][kPitch];
   const int rows = min(kTile, seg.end - seg.first);
@@ -970,11 +1003,17 @@ struct Product {
   const void* a;
   const void* b;
   const void* bias;  // forward: [G, N]
-  void* out;
-  void* sums;  // dweight: the sum of A over c, [G, N]
+  void* out;   // dweight: null for the sums alone, in the same order
+  void* sums;  // dweight: null, or the sum of A over c, [G, M]
   const int* offsets;
   long a_pitch, b_pitch;
   int G, M, N, C;  // dweight: M rows of out a group, C rows in all
+  // dweight over parts of a group's rows: 2^shift rows each (0: whole
+  // groups), whose sums go to part [.][M][N] and part_sums [.][M] unless the
+  // group has but one
+  int shift;
+  float* part;
+  float* part_sums;
 };
 
 template <typename T, int BM, int BN, int WM, int WN, int MODE, bool ASYNC>
@@ -990,7 +1029,7 @@ __global__ __launch_bounds__(WM* WN * 64) void product_kernel(Product p) {
   const int each = gridDim.x >> 3;
   int tile = blockIdx.x;
   if (tile < each * 8) tile = (tile & 7) * each + (tile >> 3);
-  const int nt = (p.N + BN - 1) / BN;
+  const int nt = p.out ? (p.N + BN - 1) / BN : 1;
   const int n0 = (tile % nt) * BN;
   tile /= nt;
 
@@ -998,20 +1037,39 @@ __global__ __launch_bounds__(WM* WN * 64) void product_kernel(Product p) {
   const T* B = reinterpret_cast<const T*>(p.b);
   int group, rows, steps;  // of out; steps of c
   long out_row, a_room, b_room;
+  bool parted = false;
   if (MODE == kDWeight) {
     const int mt = (p.M + BM - 1) / BM;
-    group = tile / mt;
+    const int unit = tile / mt;
     const int m0 = (tile % mt) * BM;
-    const int first = edge(p.offsets, group, p.G, p.C);
-    steps = edge(p.offsets, group + 1, p.G, p.C) - first;
+    int first, seg_start = 0;
+    if (p.shift) {
+      const Segment seg =
+          find_segment(p.offsets, p.G, p.C, unit, p.shift);
+      if (seg.first >= seg.end || seg.group >= p.G) return;
+      group = seg.group;
+      first = seg.first;
+      seg_start = seg.start;
+      steps = min(seg.end - first, 1 << p.shift);
+      parted = seg.end - seg.start > (1 << p.shift);
+    } else {
+      group = unit;
+      first = edge(p.offsets, group, p.G, p.C);
+      steps = edge(p.offsets, group + 1, p.G, p.C) - first;
+    }
     rows = min(BM, p.M - m0);
-    out_row = (long)group * p.M + m0;
+    out_row = (parted ? part_place(seg_start, p.shift) +
+                            ((first - seg_start) >> p.shift)
+                      : (long)group) *
+                  p.M +
+              m0;
     A += first * p.a_pitch + m0;
     B += first * p.b_pitch + n0;
     a_room = (long)(p.C - first - 1) * p.a_pitch + p.M - m0;
     b_room = (long)(p.C - first - 1) * p.b_pitch + p.N - n0;
   } else {
-    const Segment seg = find_segment<BM>(p.offsets, p.G, p.M, tile);
+    const Segment seg =
+        find_segment(p.offsets, p.G, p.M, tile, log2_of(BM));
     if (seg.first >= seg.end) return;
     group = seg.group;
     rows = min(BM, seg.end - seg.first);
@@ -1116,6 +1174,16 @@ __global__ __launch_bounds__(WM* WN * 64) void product_kernel(Product p) {
       T v[4];
 #pragma unroll
       for (int r = 0; r < 4; ++r) v[r] = (T)(acc[i][j][r] + add[r]);
+      if (MODE == kDWeight && out && parted) {
+        float* to = p.part + (out_row + m) * p.N + n0 + n;
+        if (left >= 4) {
+          __builtin_memcpy(to, &acc[i][j], 16);
+        } else {
+          for (int r = 0; r < left; ++r) to[r] = acc[i][j][r];
+        }
+        continue;
+      }
+      if (MODE == kDWeight && !out) continue;
       T* to = out + (out_row + m) * p.N + n0 + n;
       if (left >= 4) {
         __builtin_memcpy(to, v, 8);
@@ -1128,9 +1196,279 @@ __global__ __launch_bounds__(WM* WN * 64) void product_kernel(Product p) {
 #pragma unroll
     for (int i = 0; i < FM; ++i) {
       const int m = wm + i * 16 + lane;
-      if (m < rows) reinterpret_cast<T*>(p.sums)[out_row + m] = (T)sum[i][0];
+      if (m >= rows) continue;
+      if (parted)
+        p.part_sums[out_row + m] = sum[i][0];
+      else
+        reinterpret_cast<T*>(p.sums)[out_row + m] = (T)sum[i][0];
     }
   }
+}
+
+// Ends a dweight over parts: the sums of the groups that have several, in
+// their order, and zeros for groups without rows.
+template <typename T>
+__global__ __launch_bounds__(256) void finish_kernel(Product p) {
+  const int g = blockIdx.x;
+  const int start = edge(p.offsets, g, p.G, p.C);
+  const int end = edge(p.offsets, g + 1, p.G, p.C);
+  const int count = (end - start + (1 << p.shift) - 1) >> p.shift;
+  if (count == 1) return;
+  const long size = (long)p.M * p.N;
+  const long unit = part_place(start, p.shift);
+  T* out = reinterpret_cast<T*>(p.out) + g * size;
+  for (long e = (long)blockIdx.y * 256 + threadIdx.x; p.out && e < size;
+       e += (long)gridDim.y * 256) {
+    float sum = 0.f;
+    for (int u = 0; u < count; ++u) sum += p.part[(unit + u) * size + e];
+    out[e] = (T)sum;
+  }
+  if (p.sums && blockIdx.y == 0)
+    for (int m = threadIdx.x; m < p.M; m += 256) {
+      float sum = 0.f;
+      for (int u = 0; u < count; ++u) sum += p.part_sums[(unit + u) * p.M + m];
+      reinterpret_cast<T*>(p.sums)[(long)g * p.M + m] = (T)sum;
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Narrow forward products: few outputs (a keyed model's classes) or few rows
+// a group (single rows of a serving step).  The larger operand is read once,
+// straight from memory into fragments: a lane takes 16 bytes of row lane & 15
+// at the contraction's step (lane >> 4) * V, and both operands agree on which
+// steps these are, so their order in the instruction does not matter.
+// KW of the 4 waves share the contraction, the others lie along the rows.
+// ---------------------------------------------------------------------------
+template <typename T>
+struct Wide {
+  typedef T Frag __attribute__((ext_vector_type(16 / sizeof(T))));
+  static __device__ __forceinline__ f32x4 go(Frag a, Frag b, f32x4 c) {
+    if constexpr (sizeof(T) == 2) {
+      return Mma<T>::go(a, b, c);
+    } else {
+#pragma unroll
+      for (int s = 0; s < 4; ++s)
+        c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[s], b[s], c, 0, 0, 0);
+      return c;
+    }
+  }
+  static __device__ __forceinline__ Frag load(const T* p) {
+    Frag v;
+    __builtin_memcpy(&v, p, 16);
+    return v;
+  }
+  static __device__ __forceinline__ Frag load(const T* p, int n) {
+    Frag v;
+#pragma unroll
+    for (int i = 0; i < (int)(16 / sizeof(T)); ++i)
+      v[i] = i < n ? p[i] : (T)0.f;
+    return v;
+  }
+};
+
+template <typename T, int MF, int NF, int KW>
+__global__ __launch_bounds__(256) void narrow_kernel(Product p, bool by_row) {
+  constexpr int V = 16 / sizeof(T), kChunk = 4 * V;
+  constexpr int BM = 4 / KW * MF * 16, BN = NF * 16;
+  const Segment seg =
+      by_row ? find_segment_at(p.offsets, p.G, p.M, blockIdx.x, log2_of(BM))
+             : find_segment(p.offsets, p.G, p.M, blockIdx.x, log2_of(BM));
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
+  const int part = wave % KW;
+  const int row0 = seg.first + wave / KW * MF * 16;
+  const int n0 = blockIdx.y * BN;
+  if (KW == 1 ? row0 >= seg.end : seg.first >= seg.end) return;
+  f32x4 acc[MF][NF] = {};
+  if (seg.group < p.G) {
+    // rows and outputs past the end read the last one's values, and are not
+    // stored
+    const T *a[MF], *b[NF];
+#pragma unroll
+    for (int i = 0; i < MF; ++i)
+      a[i] = reinterpret_cast<const T*>(p.a) +
+             min(row0 + i * 16 + r, seg.end - 1) * p.a_pitch + q * V;
+#pragma unroll
+    for (int j = 0; j < NF; ++j)
+      b[j] = reinterpret_cast<const T*>(p.b) +
+             ((long)seg.group * p.N + min(n0 + j * 16 + r, p.N - 1)) * p.C +
+             q * V;
+    const int whole = p.C / kChunk * kChunk;
+    int c = part * kChunk;
+#pragma unroll 4
+    for (; c < whole; c += KW * kChunk) {
+      typename Wide<T>::Frag fa[MF], fb[NF];
+#pragma unroll
+      for (int i = 0; i < MF; ++i) fa[i] = Wide<T>::load(a[i] + c);
+#pragma unroll
+      for (int j = 0; j < NF; ++j) fb[j] = Wide<T>::load(b[j] + c);
+#pragma unroll
+      for (int i = 0; i < MF; ++i)
+#pragma unroll
+        for (int j = 0; j < NF; ++j)
+          acc[i][j] = Wide<T>::go(fb[j], fa[i], acc[i][j]);
+    }
+    if (c == whole && whole < p.C) {
+      const int left = p.C - whole - q * V;
+      typename Wide<T>::Frag fa[MF], fb[NF];
+#pragma unroll
+      for (int i = 0; i < MF; ++i) fa[i] = Wide<T>::load(a[i] + c, left);
+#pragma unroll
+      for (int j = 0; j < NF; ++j) fb[j] = Wide<T>::load(b[j] + c, left);
+#pragma unroll
+      for (int i = 0; i < MF; ++i)
+#pragma unroll
+        for (int j = 0; j < NF; ++j)
+          acc[i][j] = Wide<T>::go(fb[j], fa[i], acc[i][j]);
+    }
+  }
+  if constexpr (KW > 1) {
+    __shared__ f32x4 sums[4][MF * NF][64];
+#pragma unroll
+    for (int i = 0; i < MF; ++i)
+#pragma unroll
+      for (int j = 0; j < NF; ++j) sums[wave][i * NF + j][lane] = acc[i][j];
+    __syncthreads();
+    if (part) return;
+#pragma unroll
+    for (int w = 1; w < KW; ++w)
+#pragma unroll
+      for (int i = 0; i < MF; ++i)
+#pragma unroll
+        for (int j = 0; j < NF; ++j)
+          acc[i][j] += sums[wave + w][i * NF + j][lane];
+  }
+  const T* bias = reinterpret_cast<const T*>(p.bias);
+#pragma unroll
+  for (int j = 0; j < NF; ++j) {
+    const int n = n0 + j * 16 + q * 4;
+    const int left = p.N - n;
+    if (left <= 0) continue;
+    float add[4] = {};
+    if (bias && seg.group < p.G) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (e < left) add[e] = to_f(bias[(long)seg.group * p.N + n + e]);
+    }
+#pragma unroll
+    for (int i = 0; i < MF; ++i) {
+      const int m = row0 + i * 16 + r;
+      if (m >= seg.end) continue;
+      T v[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = (T)(acc[i][j][e] + add[e]);
+      T* to = reinterpret_cast<T*>(p.out) + (long)m * p.N + n;
+      if (left >= 4) {
+        __builtin_memcpy(to, v, sizeof(v));
+      } else {
+        for (int e = 0; e < left; ++e) to[e] = v[e];
+      }
+    }
+  }
+}
+
+// float32 dweight with few outputs: dw[g, n, f] for 16 * NF outputs.  A lane
+// takes 4 columns f = 4 * (lane & 15) + e of the row (lane >> 4) * 4 + i, which
+// are four fragments' values at once.  KW of the 4 waves share the rows, the
+// others lie along f.
+template <int NF, int KW>
+__global__ __launch_bounds__(256) void narrow_dweight_kernel(Product p) {
+  constexpr int BF = 4 / KW * 64;
+  const Segment seg = find_segment(p.offsets, p.G, p.C, blockIdx.x, p.shift);
+  if (seg.first >= seg.end || seg.group >= p.G) return;
+  const int end = min(seg.end, seg.first + (1 << p.shift));
+  const bool parted = seg.end - seg.start > (1 << p.shift);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
+  const int part = wave % KW;
+  const int f = blockIdx.y * BF + wave / KW * 64 + r * 4;
+  const int n0 = blockIdx.z * NF * 16;
+  const int left = p.N - f;
+  const bool sums = p.sums && blockIdx.y == 0 && wave / KW == 0;
+  const float* a = reinterpret_cast<const float*>(p.a);
+  const float* b = reinterpret_cast<const float*>(p.b) + f;
+  int n[NF];
+#pragma unroll
+  for (int j = 0; j < NF; ++j) n[j] = min(n0 + j * 16 + r, p.M - 1);
+  f32x4 acc[NF][4] = {};
+  f32x4 sum[NF] = {};
+#pragma unroll 2
+  for (int s = seg.first + part * 16; s < end; s += KW * 16) {
+    float fa[NF][4];
+    f32x4 fb[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int row = s + q * 4 + i;
+      const bool in = row < end;
+      const long at = in ? row : end - 1;
+#pragma unroll
+      for (int j = 0; j < NF; ++j) {
+        const float v = a[at * p.a_pitch + n[j]];
+        fa[j][i] = in ? v : 0.f;
+      }
+      f32x4 v = {};
+      if (left >= 4) {
+        __builtin_memcpy(&v, b + at * p.b_pitch, 16);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 3; ++e)
+          if (e < left) v[e] = b[at * p.b_pitch + e];
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) fb[i][e] = in ? v[e] : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < NF; ++j) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          acc[j][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(
+              fa[j][i], fb[i][e], acc[j][e], 0, 0, 0);
+        if (sums)
+          sum[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(fa[j][i], 1.f, sum[j],
+                                                        0, 0, 0);
+      }
+  }
+  if constexpr (KW > 1) {
+    __shared__ f32x4 all[4][NF * 5][64];
+#pragma unroll
+    for (int j = 0; j < NF; ++j) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) all[wave][j * 5 + e][lane] = acc[j][e];
+      all[wave][j * 5 + 4][lane] = sum[j];
+    }
+    __syncthreads();
+    if (part) return;
+#pragma unroll
+    for (int w = 1; w < KW; ++w)
+#pragma unroll
+      for (int j = 0; j < NF; ++j) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          acc[j][e] += all[wave + w][j * 5 + e][lane];
+        sum[j] += all[wave + w][j * 5 + 4][lane];
+      }
+  }
+  const long out_row =
+      (parted ? part_place(seg.start, p.shift) +
+                    ((seg.first - seg.start) >> p.shift)
+              : (long)seg.group) *
+      p.M;
+  float* out = parted && p.out ? p.part : reinterpret_cast<float*>(p.out);
+  float* out_sums = parted ? p.part_sums : reinterpret_cast<float*>(p.sums);
+#pragma unroll
+  for (int j = 0; j < NF; ++j)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int m = n0 + j * 16 + q * 4 + i;
+      if (m >= p.M) continue;
+      float* to = out + (out_row + m) * p.N + f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (p.out && e < left) to[e] = acc[j][e][i];
+      if (sums && r == 0) out_sums[out_row + m] = sum[j][i];
+    }
 }
 
 // Buffer loads to LDS take addresses of whole words.
@@ -1139,24 +1477,115 @@ bool whole_words(const T* p, long pitch) {
   return (reinterpret_cast<uintptr_t>(p) & 3) == 0 && (pitch & 1) == 0;
 }
 
+unsigned grid_of(long blocks, int threads) {
+  TORCH_CHECK(blocks * threads < (1ll << 32), "too many tiles");
+  return (unsigned)blocks;
+}
+
+template <typename T>
+bool narrow_launch(const Product& p) {
+  const long rows = p.M / std::min(p.G, p.M);
+  auto go = [&](auto kern, int bm, int bn) {
+    const bool by_row = p.M < p.M / bm + p.G + 1;
+    const long tiles = by_row ? p.M : p.M / bm + p.G + 1;
+    dim3 grid(grid_of(tiles, 256), (p.N + bn - 1) / bn);
+    TORCH_CHECK(grid.y < 65536, "rows are too wide");
+    kern<<<grid, 256, 0, stream_now()>>>(p, by_row);
+    check_launch();
+    return true;
+  };
+  if (rows <= 16) return go(narrow_kernel<T, 1, 1, 4>, 16, 16);
+  if (p.N <= 16) return go(narrow_kernel<T, 4, 1, 1>, 256, 16);
+  if (p.N <= 32) return go(narrow_kernel<T, 4, 2, 1>, 256, 32);
+  if (p.N <= 64) return go(narrow_kernel<T, 4, 4, 1>, 256, 64);
+  return false;
+}
+
+// Parts of a group's rows, so that `tiles` outputs a group make about `want`
+// blocks of work that are alike.
+int part_shift(long rows, long tiles, long want) {
+  int shift = 8;
+  while (shift < 30 && (rows * tiles >> shift) > want) ++shift;
+  return shift;
+}
+
+struct Parts {
+  at::Tensor part, sums;
+};
+
+Parts take_parts(Product& p, at::TensorOptions opt) {
+  Parts parts;
+  const int64_t units = 2 * (((int64_t)p.C >> p.shift) + 1);
+  if (p.out) {
+    parts.part = at::empty({units, p.M, p.N}, opt.dtype(at::kFloat));
+    p.part = parts.part.data_ptr<float>();
+  }
+  if (p.sums) {
+    parts.sums = at::empty({units, p.M}, opt.dtype(at::kFloat));
+    p.part_sums = parts.sums.data_ptr<float>();
+  }
+  return parts;
+}
+
+template <typename T>
+void finish_launch(const Product& p) {
+  const long size = (long)p.M * p.N;
+  dim3 grid(grid_of(p.G, 256), std::max(1l, std::min(1024l, size / 1024)));
+  finish_kernel<T><<<grid, 256, 0, stream_now()>>>(p);
+  check_launch();
+}
+
 template <typename T, int MODE>
-void product_launch(const Product& p) {
+void product_launch(Product p, at::TensorOptions opt) {
+  if (MODE == kForward && narrow_launch<T>(p)) return;
   const bool async = whole_words((const T*)p.a, p.a_pitch) &&
                      whole_words((const T*)p.b, p.b_pitch) &&
                      // the weights of a group may begin at an odd value
                      (MODE == kDWeight || ((long)p.N * p.C) % 2 == 0);
   auto go = [&](auto kern, int bm, int bn, int threads) {
-    const long mt = MODE == kDWeight ? (long)p.G * ((p.M + bm - 1) / bm)
-                                     : (long)p.M / bm + p.G + 1;
-    const long blocks = mt * ((p.N + bn - 1) / bn);
-    TORCH_CHECK(blocks * threads < (1ll << 32), "too many tiles");
-    kern<<<(unsigned)blocks, threads, 0, stream_now()>>>(p);
+    const long m_tiles = (p.M + bm - 1) / bm, n_tiles = (p.N + bn - 1) / bn;
+    long mt = (long)p.M / bm + p.G + 1;
+    Parts parts;
+    if (MODE == kDWeight) {
+      mt = p.G * m_tiles;
+      if (mt * n_tiles < 512) {
+        p.shift = part_shift(p.C, m_tiles * n_tiles, 512);
+        parts = take_parts(p, opt);
+        mt = ((p.C >> p.shift) + p.G + 1) * m_tiles;
+      }
+    }
+    const long nt = p.out ? n_tiles : 1;
+    kern<<<grid_of(mt * nt, threads), threads, 0, stream_now()>>>(p);
+    check_launch();
+    if (MODE == kDWeight && p.shift) finish_launch<T>(p);
+  };
+  if (!async)
+    go(product_kernel<T, 128, 128, 2, 2, MODE, false>, 128, 128, 256);
+  else if (p.M <= 128 || p.N <= 128)
+    go(product_kernel<T, 128, 128, 2, 2, MODE, true>, 128, 128, 256);
+  else
+    go(product_kernel<T, 256, 256, 2, 4, MODE, true>, 256, 256, 512);
+}
+
+void narrow_dweight_launch(Product p, at::TensorOptions opt) {
+  const int kw = p.N <= 64 ? 4 : 1, bf = 4 / kw * 64;
+  const int nf = p.M <= 16 ? 1 : 2;
+  const long n_tiles =
+      ((p.M + nf * 16 - 1) / (nf * 16)) * (long)((p.N + bf - 1) / bf);
+  p.shift = part_shift(p.C, n_tiles, 2048);
+  Parts parts = take_parts(p, opt);
+  dim3 grid(grid_of(((long)p.C >> p.shift) + p.G + 1, 256),
+            p.out ? (p.N + bf - 1) / bf : 1, (p.M + nf * 16 - 1) / (nf * 16));
+  TORCH_CHECK(grid.y < 65536 && grid.z < 65536, "rows are too wide");
+  auto go = [&](auto kern) {
+    kern<<<grid, 256, 0, stream_now()>>>(p);
     check_launch();
   };
-  if (async)
-    go(product_kernel<T, 256, 256, 2, 4, MODE, true>, 256, 256, 512);
+  if (kw == 4)
+    nf == 1 ? go(narrow_dweight_kernel<1, 4>) : go(narrow_dweight_kernel<2, 4>);
   else
-    go(product_kernel<T, 128, 128, 2, 2, MODE, false>, 128, 128, 256);
+    nf == 1 ? go(narrow_dweight_kernel<1, 1>) : go(narrow_dweight_kernel<2, 1>);
+  finish_launch<float>(p);
 }
 
 void check_product(const at::Tensor& a, const at::Tensor& weight,
@@ -1201,15 +1630,22 @@ at::Tensor product(const at::Tensor& a_in, const at::Tensor& weight,
         Product p{a.data_ptr(), weight.data_ptr(),
                   bias ? bias->data_ptr() : nullptr, out.data_ptr(), nullptr,
                   offsets.data_ptr<int>(), a.stride(0),
-                  transposed ? N : C, G, M, N, C};
+                  transposed ? N : C, G, M, N, C, 0, nullptr, nullptr};
         if (transposed)
-          product_launch<T, kDRows>(p);
+          product_launch<T, kDRows>(p, a.options());
         else
-          product_launch<T, kForward>(p);
+          product_launch<T, kForward>(p, a.options());
       }
     });
     return out;
   }
+  if (!transposed &&
+      narrow_launch<float>(
+          Product{a.data_ptr(), weight.data_ptr(),
+                  bias ? bias->data_ptr() : nullptr, out.data_ptr(), nullptr,
+                  offsets.data_ptr<int>(), a.stride(0), C, G, M, N, C, 0,
+                  nullptr, nullptr}))
+    return out;
   SKA_TYPES(a.scalar_type(), [&] {
     dim3 grid(M / kTile + G + 1, (N + kTile - 1) / kTile);
     TORCH_CHECK(grid.y < 65536, "rows are too wide");
@@ -1235,9 +1671,12 @@ at::Tensor grouped_linear_drows(const at::Tensor& dy,
   return product(dy, weight, offsets, c10::nullopt, true);
 }
 
-std::tuple<at::Tensor, c10::optional<at::Tensor>> grouped_linear_dweight(
-    const at::Tensor& dy_in, const at::Tensor& rows_in,
-    const at::Tensor& offsets, bool need_bias) {
+// (dweight, dbias); one that is not asked for comes back undefined.  The bias
+// alone is summed in the same order as together with the weights.
+std::tuple<c10::optional<at::Tensor>, c10::optional<at::Tensor>>
+grouped_linear_dweight(const at::Tensor& dy_in, const at::Tensor& rows_in,
+                       const at::Tensor& offsets, bool need_weight,
+                       bool need_bias) {
   TORCH_CHECK(dy_in.is_cuda() && dy_in.dim() == 2 && rows_in.dim() == 2 &&
                   rows_in.device() == dy_in.device() &&
                   rows_in.dtype() == dy_in.dtype() &&
@@ -1255,29 +1694,36 @@ std::tuple<at::Tensor, c10::optional<at::Tensor>> grouped_linear_dweight(
   at::Tensor dy = packed_rows(dy_in), x = packed_rows(rows_in);
   const int G = (int)offsets.numel() - 1, M = (int)dy.size(0);
   const int N = (int)dy.size(1), F = (int)x.size(1);
-  at::Tensor dw = at::empty({G, N, F}, dy.options());
-  c10::optional<at::Tensor> db;
+  c10::optional<at::Tensor> dw, db;
+  if (need_weight) dw = at::empty({G, N, F}, dy.options());
   if (need_bias) db = at::empty({G, N}, dy.options());
-  if (N == 0) return {dw, db};
-  if (dy.scalar_type() != at::kFloat && F > 0 && M > 0) {
-    SKA_TYPES(dy.scalar_type(), [&] {
-      if constexpr (sizeof(T) == 2)
-        product_launch<T, kDWeight>(
-            Product{dy.data_ptr(), x.data_ptr(), nullptr, dw.data_ptr(),
-                    db ? db->data_ptr() : nullptr, offsets.data_ptr<int>(),
-                    dy.stride(0), x.stride(0), G, N, F, M});
-    });
+  if (N == 0 || (!need_weight && !need_bias)) return {dw, db};
+  if (M == 0) {
+    if (dw) dw->zero_();
+    if (db) db->zero_();
     return {dw, db};
   }
+  if (F == 0 && !need_bias) return {dw, db};
+  // rows of no width leave the bias: any other operand does for its sums
+  const at::Tensor& b = F ? x : dy;
+  Product p{dy.data_ptr(), b.data_ptr(), nullptr,
+            F && dw ? dw->data_ptr() : nullptr, db ? db->data_ptr() : nullptr,
+            offsets.data_ptr<int>(), dy.stride(0), b.stride(0), G, N,
+            F ? F : N, M, 0, nullptr, nullptr};
   SKA_TYPES(dy.scalar_type(), [&] {
-    // at least one column tile, which sums the bias where F is 0
-    dim3 grid(G, (N + kTile - 1) / kTile, std::max(1, (F + kTile - 1) / kTile));
-    TORCH_CHECK(grid.y < 65536 && grid.z < 65536, "rows are too wide");
-    weights_plain_kernel<T><<<grid, 256, 0, stream_now()>>>(
-        ptr<T>(dy), dy.stride(0), ptr<T>(x), x.stride(0),
-        offsets.data_ptr<int>(), G, M, N, F, ptr<T>(dw),
-        db ? ptr<T>(*db) : nullptr);
-    check_launch();
+    if constexpr (sizeof(T) == 2) {
+      product_launch<T, kDWeight>(p, dy.options());
+    } else if (N <= 64 || !p.out) {
+      narrow_dweight_launch(p, dy.options());
+    } else {
+      dim3 grid(G, (N + kTile - 1) / kTile, (F + kTile - 1) / kTile);
+      TORCH_CHECK(grid.y < 65536 && grid.z < 65536, "rows are too wide");
+      weights_plain_kernel<T><<<grid, 256, 0, stream_now()>>>(
+          ptr<T>(dy), dy.stride(0), ptr<T>(x), x.stride(0),
+          offsets.data_ptr<int>(), G, M, N, F, ptr<T>(*dw),
+          db ? ptr<T>(*db) : nullptr);
+      check_launch();
+    }
   });
   return {dw, db};
 }

@@ -18,10 +18,10 @@ from ..grouped_rows import (_kernels, combine_rows, gather_rows, group_rows,
 __all__ = ["KeyedLinearExecutor", "keyed_scores"]
 
 
-def _sums(values, rows, offsets):
+def _sums(values, offsets):
     """The sum of each group's run of rows [G, C]."""
     _, total = _kernels(values).grouped_linear_dweight(
-        values, rows[:, :0], offsets, True)
+        values, values, offsets, False, True)
     return total
 
 
@@ -99,10 +99,10 @@ class KeyedLinearExecutor:
             else:
                 d = z - t
                 le = 0.5 * d * d
-            cur = _sums(le, rows, offsets) * inv_n
+            cur = _sums(le, offsets) * inv_n
             now = active & (epoch < limit)
             n_iter = torch.where(now, epoch + 1, n_iter)
-            g, gb = k.grouped_linear_dweight(d, rows, offsets, True)
+            g, gb = k.grouped_linear_dweight(d, rows, offsets, True, True)
             g = g * inv_n[..., None] + l2[..., None] * W \
                 + l1[..., None] * torch.sign(W)
             gb = gb * inv_n * intercept

@@ -257,6 +257,9 @@ PRODUCTS = [  # M, G, N, F, offsets
     (257, 300, 40, 24, "ragged"), (500, 3, 200, 130, "first"),
     (200, 6, 72, 96, "nobody"), (1025, 5, 129, 257, "tail"),
     (900, 2, 264, 520, "last"), (700, 11, 384, 136, "ragged"),
+    (1500, 3, 5, 70, "ragged"), (3000, 40, 3, 260, "ragged"),
+    (2000, 2, 40, 33, "first"), (1100, 600, 20, 9, "tail"),
+    (40, 90, 300, 48, "ragged"), (1030, 1, 61, 2056, "even"),
 ]
 
 
