@@ -17,6 +17,7 @@
 
 #include <algorithm>
 #include <tuple>
+#include <type_traits>
 
 namespace {
 
@@ -126,7 +127,7 @@ __global__ __launch_bounds__(256) void sort_count_kernel(
               1);
   __syncthreads();
   for (int b = threadIdx.x; b < bins; b += 256)
-    table[(long)b * blocks + blockIdx.x] = count[b];
+    table[(long)blockIdx.x * bins + b] = count[b];
 }
 
 __device__ __forceinline__ int wave_scan(int v, int lane) {
@@ -138,22 +139,32 @@ __device__ __forceinline__ int wave_scan(int v, int lane) {
   return v;
 }
 
-// One wave a bin: its counts become the numbers of such entries in the
-// blocks before, and total[bin] their sum.
+// A bin's counts become the numbers of such entries in the blocks before, and
+// total[bin] their sum.  64 bins a block, whose 4 waves share the blocks.
 __global__ __launch_bounds__(256) void sort_scan_kernel(
     int bins, int blocks, int* __restrict__ table, int* __restrict__ total) {
-  const int lane = threadIdx.x & 63;
-  const int bin = blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (bin >= bins) return;
-  int* row = table + (long)bin * blocks;
+  __shared__ int sums[4][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int bin = blockIdx.x * 64 + lane;
+  const int part = (blocks + 3) / 4;
+  const int first = wave * part, last = min(blocks, first + part);
   int sum = 0;
-  for (int b = 0; b < blocks; b += 64) {
-    int v = b + lane < blocks ? row[b + lane] : 0;
-    int s = wave_scan(v, lane);
-    if (b + lane < blocks) row[b + lane] = sum + s - v;
-    sum += __shfl(s, 63);
+  if (bin < bins) {
+#pragma unroll 8
+    for (int b = first; b < last; ++b) sum += table[(long)b * bins + bin];
   }
-  if (lane == 0) total[bin] = sum;
+  sums[wave][lane] = sum;
+  __syncthreads();
+  int at = 0;
+  for (int w = 0; w < wave; ++w) at += sums[w][lane];
+  if (bin >= bins) return;
+  if (wave == 3) total[bin] = at + sum;
+#pragma unroll 8
+  for (int b = first; b < last; ++b) {
+    const int n = table[(long)b * bins + bin];
+    table[(long)b * bins + bin] = at;
+    at += n;
+  }
 }
 
 // The bins' first positions; where one pass sorts, these are the offsets.
@@ -199,7 +210,7 @@ __global__ __launch_bounds__(256) void sort_place_kernel(
               1);
   __syncthreads();
   for (int b = threadIdx.x; b < bins; b += 256) {
-    int at = base[b] + table[(long)b * blocks + blockIdx.x];
+    int at = base[b] + table[(long)blockIdx.x * bins + b];
 #pragma unroll
     for (int w = 0; w < kSortWaves; ++w) {
       int n = place[w * bins + b];
@@ -257,11 +268,12 @@ void sort_launch(const I* ids, int M, int G, int* offsets, int* slots,
   const bool one = G + 1 <= kBins;
   const int digit = one ? bits : (bits + 1) / 2;
   const int mask = (1 << digit) - 1;
-  // 2048 entries a block at least, 1024 blocks at most
-  int tile = 2048;
-  while ((long)tile * 1024 < M) tile *= 2;
-  const int blocks = (int)(((long)M + tile - 1) / tile);
   const int bins = one ? G + 1 : 1 << digit;
+  // 2048 entries a block at least, and not fewer than it has counters; 1024
+  // blocks at most
+  int tile = 2048;
+  while (tile < bins || (long)tile * 1024 < M) tile *= 2;
+  const int blocks = (int)(((long)M + tile - 1) / tile);
   at::Tensor table = at::empty({(int64_t)bins * blocks + 2 * bins}, opt);
   int* tab = table.data_ptr<int>();
   int* total = tab + (long)bins * blocks;
@@ -279,7 +291,7 @@ void sort_launch(const I* ids, int M, int G, int* offsets, int* slots,
     constexpr bool F = decltype(first)::value, L = decltype(last)::value;
     sort_count_kernel<I, F><<<blocks, 256, lds, s>>>(
         ids, k0, M, G, shift, mask, bins, tile, blocks, tab);
-    sort_scan_kernel<<<(bins + 3) / 4, 256, 0, s>>>(bins, blocks, tab, total);
+    sort_scan_kernel<<<(bins + 63) / 64, 256, 0, s>>>(bins, blocks, tab, total);
     sort_base_kernel<<<1, 1024, 0, s>>>(bins, total, base);
     sort_place_kernel<I, F, L><<<blocks, 256, lds * kSortWaves, s>>>(
         ids, k0, e0, M, G, shift, mask, digit, bins, tile, blocks, tab, base,
@@ -338,17 +350,22 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> group_rows(
 // start at odd addresses, which the loads and stores here may have; the
 // elements behind the last whole vector go one by one.
 // ---------------------------------------------------------------------------
+// 16 bytes that may begin at any value: one load or store instruction.
+typedef unsigned Bytes16 __attribute__((ext_vector_type(4), aligned(2)));
+
 template <typename T>
 struct Vec {
   static constexpr int N = 16 / sizeof(T);
-  T v[N];
+  typedef T Values __attribute__((ext_vector_type(16 / sizeof(T))));
+  Values v;
 };
 
 template <typename T>
 __device__ __forceinline__ Vec<T> load_vec(const T* p, int n) {
   Vec<T> r;
   if (n >= Vec<T>::N) {
-    __builtin_memcpy(&r, p, 16);
+    r.v = __builtin_bit_cast(decltype(r.v),
+                             *reinterpret_cast<const Bytes16*>(p));
   } else {
 #pragma unroll
     for (int i = 0; i < Vec<T>::N; ++i) r.v[i] = i < n ? p[i] : (T)0.f;
@@ -359,7 +376,7 @@ __device__ __forceinline__ Vec<T> load_vec(const T* p, int n) {
 template <typename T>
 __device__ __forceinline__ void store_vec(T* p, const Vec<T>& r, int n) {
   if (n >= Vec<T>::N) {
-    __builtin_memcpy(p, &r, 16);
+    *reinterpret_cast<Bytes16*>(p) = __builtin_bit_cast(Bytes16, r.v);
   } else {
 #pragma unroll
     for (int i = 0; i < Vec<T>::N; ++i)
@@ -367,104 +384,230 @@ __device__ __forceinline__ void store_vec(T* p, const Vec<T>& r, int n) {
   }
 }
 
+template <int N>
+using Count = std::integral_constant<int, N>;
+
+// A lane's share of a row of F values: `some(at, Count<U>)` for U vectors at
+// `at`, `at` + step, ..., as many in flight; then `one(at)` for the values
+// behind the last whole vector, a lane each.
+template <int V, int U, typename Some, typename One>
+__device__ __forceinline__ void walk_row(int F, int lane, int lanes,
+                                         Some some, One one) {
+  const int whole = F / V * V, step = lanes * V;
+  int at = lane * V;
+  for (; at + (U - 1) * step < whole; at += U * step) some(at, Count<U>{});
+  for (; at < whole; at += step) some(at, Count<1>{});
+  for (int e = whole + lane; e < F; e += lanes) one(e);
+}
+
 template <typename T>
+__device__ __forceinline__ Vec<T> get(const T* p) {
+  Vec<T> r;
+  r.v = __builtin_bit_cast(decltype(r.v),
+                           *reinterpret_cast<const Bytes16*>(p));
+  return r;
+}
+
+template <typename T>
+__device__ __forceinline__ void put(T* p, const Vec<T>& r) {
+  *reinterpret_cast<Bytes16*>(p) = __builtin_bit_cast(Bytes16, r.v);
+}
+
+template <typename T, int U>
 __global__ __launch_bounds__(256) void gather_kernel(
     const T* __restrict__ x, long x_pitch, const int* __restrict__ slots,
     const int* __restrict__ kept_end, int T_rows, int k, int F, int lanes,
     T* __restrict__ out) {
+  constexpr int V = Vec<T>::N;
   const int per = 256 / lanes;
-  const int t = blockIdx.x * per + threadIdx.x / lanes;
-  if (t >= T_rows) return;
   const int M = T_rows * k;
   const int S = clampi(*kept_end, 0, M);
-  constexpr int V = Vec<T>::N;
-  const T* src = x + (long)t * x_pitch;
-  for (int c = (threadIdx.x % lanes) * V; c < F; c += lanes * V) {
-    const Vec<T> v = load_vec(src + c, F - c);
-    for (int j = 0; j < k; ++j) {
-      const int s = slots[(long)t * k + j];
-      if ((unsigned)s >= (unsigned)M) continue;
-      Vec<T> w = v;
-      if (s >= S) {
+  const int step = lanes * V;
+  for (long t = (long)blockIdx.x * per + threadIdx.x / lanes; t < T_rows;
+       t += (long)gridDim.x * per) {
+    const T* src = x + t * x_pitch;
+    walk_row<V, U>(
+        F, threadIdx.x % lanes, lanes,
+        [&](int at, auto n) {
+          constexpr int N = decltype(n)::value;
+          Vec<T> v[N];
 #pragma unroll
-        for (int i = 0; i < V; ++i) w.v[i] = (T)0.f;
-      }
-      store_vec(out + (long)s * F + c, w, F - c);
-    }
+          for (int u = 0; u < N; ++u) v[u] = get(src + at + u * step);
+          for (int j = 0; j < k; ++j) {
+            const int s = slots[t * k + j];
+            if ((unsigned)s >= (unsigned)M) continue;
+            T* to = out + (long)s * F + at;
+#pragma unroll
+            for (int u = 0; u < N; ++u) {
+              Vec<T> w = v[u];
+              if (s >= S) w.v = (T)0.f;
+              put(to + u * step, w);
+            }
+          }
+        },
+        [&](int at) {
+          const T v = src[at];
+          for (int j = 0; j < k; ++j) {
+            const int s = slots[t * k + j];
+            if ((unsigned)s < (unsigned)M)
+              out[(long)s * F + at] = s < S ? v : (T)0.f;
+          }
+        });
   }
 }
 
 // y[t] = sum over the kept entries of w[t, j] * rows[slots[t, j]], in the
-// order of j and in 32 bits.  W = void: no weights.
-template <typename T, typename W>
+// order of j and in 32 bits; J rows are read at a time.
+template <typename T, typename W, int J, int U>
 __global__ __launch_bounds__(256) void combine_kernel(
     const T* __restrict__ rows, long pitch, const int* __restrict__ slots,
     const int* __restrict__ kept_end, const W* __restrict__ weights,
     int T_rows, int k, int F, int lanes, T* __restrict__ y) {
-  const int per = 256 / lanes;
-  const int t = blockIdx.x * per + threadIdx.x / lanes;
-  if (t >= T_rows) return;
-  const int S = clampi(*kept_end, 0, T_rows * k);
   constexpr int V = Vec<T>::N;
-  for (int c = (threadIdx.x % lanes) * V; c < F; c += lanes * V) {
-    float acc[V] = {};
-    for (int j = 0; j < k; ++j) {
-      const int s = slots[(long)t * k + j];
-      if ((unsigned)s >= (unsigned)S) continue;
-      const float w = weights ? (float)weights[(long)t * k + j] : 1.f;
-      const Vec<T> v = load_vec(rows + (long)s * pitch + c, F - c);
+  const int per = 256 / lanes;
+  const int S = clampi(*kept_end, 0, T_rows * k);
+  const int step = lanes * V;
+  for (long t = (long)blockIdx.x * per + threadIdx.x / lanes; t < T_rows;
+       t += (long)gridDim.x * per) {
+    walk_row<V, U>(
+        F, threadIdx.x % lanes, lanes,
+        [&](int at, auto n) {
+          constexpr int N = decltype(n)::value;
+          float acc[N][V] = {};
+          for (int j0 = 0; j0 < k; j0 += J) {
+            bool kept[J];
+            float w[J];
+            Vec<T> v[J][N];
 #pragma unroll
-      for (int i = 0; i < V; ++i) acc[i] += w * to_f(v.v[i]);
-    }
-    Vec<T> o;
+            for (int j = 0; j < J; ++j) {
+              const long e = t * k + j0 + j;
+              const int s = j0 + j < k ? slots[e] : -1;
+              kept[j] = (unsigned)s < (unsigned)S;
+              w[j] = kept[j] && weights ? (float)weights[e] : 1.f;
+              // an entry that is left out reads the first row, for nothing
+              const T* src = rows + (kept[j] ? (long)s * pitch : 0) + at;
 #pragma unroll
-    for (int i = 0; i < V; ++i) o.v[i] = (T)acc[i];
-    store_vec(y + (long)t * F + c, o, F - c);
+              for (int u = 0; u < N; ++u) v[j][u] = get(src + u * step);
+            }
+#pragma unroll
+            for (int j = 0; j < J; ++j)
+#pragma unroll
+              for (int u = 0; u < N; ++u)
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                  const float next = acc[u][i] + w[j] * to_f(v[j][u].v[i]);
+                  acc[u][i] = kept[j] ? next : acc[u][i];
+                }
+          }
+#pragma unroll
+          for (int u = 0; u < N; ++u) {
+            Vec<T> o;
+#pragma unroll
+            for (int i = 0; i < V; ++i) o.v[i] = (T)acc[u][i];
+            put(y + t * F + at + u * step, o);
+          }
+        },
+        [&](int at) {
+          float acc = 0.f;
+          for (int j = 0; j < k; ++j) {
+            const int s = slots[t * k + j];
+            if ((unsigned)s >= (unsigned)S) continue;
+            const float w = weights ? (float)weights[t * k + j] : 1.f;
+            acc += w * to_f(rows[(long)s * pitch + at]);
+          }
+          y[t * F + at] = (T)acc;
+        });
   }
 }
 
-// Backward of combine, in row order: dy[t] is read once, each of its k rows
+// Backward of combine, in row order: dy[t] is read once for J rows, each row
 // once; drows (where asked for) and the dot products leave with them.
-template <typename T, typename W>
+template <typename T, typename W, int J, int U>
 __global__ __launch_bounds__(256) void combine_back_kernel(
     const T* __restrict__ dy, long dy_pitch, const T* __restrict__ rows,
     long pitch, const int* __restrict__ slots,
     const int* __restrict__ kept_end, const W* __restrict__ weights,
     int T_rows, int k, int F, int lanes, T* __restrict__ drows,
     W* __restrict__ dw) {
+  constexpr int V = Vec<T>::N;
   const int per = 256 / lanes;
-  const int t = blockIdx.x * per + threadIdx.x / lanes;
-  const bool in = t < T_rows;
   const int M = T_rows * k;
   const int S = clampi(*kept_end, 0, M);
-  constexpr int V = Vec<T>::N;
   const int lane = threadIdx.x % lanes;
-  for (int j = 0; j < k; ++j) {
-    const int s = in ? slots[(long)t * k + j] : -1;
-    const bool kept = (unsigned)s < (unsigned)S;
-    const float w =
-        !kept ? 0.f : (weights ? (float)weights[(long)t * k + j] : 1.f);
-    float dot = 0.f;
-    if ((unsigned)s < (unsigned)M) {
-      for (int c = lane * V; c < F; c += lanes * V) {
-        const Vec<T> d = load_vec(dy + (long)t * dy_pitch + c, F - c);
-        if (dw && kept) {
-          const Vec<T> r = load_vec(rows + (long)s * pitch + c, F - c);
+  const int step = lanes * V;
+  for (long t0 = (long)blockIdx.x * per; t0 < T_rows;
+       t0 += (long)gridDim.x * per) {
+    const long t = t0 + threadIdx.x / lanes;
+    const bool in = t < T_rows;
+    for (int j0 = 0; j0 < k; j0 += J) {
+      int s[J];
+      float w[J], dot[J] = {};
 #pragma unroll
-          for (int i = 0; i < V; ++i) dot += to_f(d.v[i]) * to_f(r.v[i]);
-        }
-        if (drows) {
-          Vec<T> o;
+      for (int j = 0; j < J; ++j) {
+        s[j] = in && j0 + j < k ? slots[t * k + j0 + j] : -1;
+        w[j] = 1.f;
+        if (weights && (unsigned)s[j] < (unsigned)S)
+          w[j] = (float)weights[t * k + j0 + j];
+      }
+      if (in)
+        walk_row<V, U>(
+            F, lane, lanes,
+            [&](int at, auto n) {
+              constexpr int N = decltype(n)::value;
+              Vec<T> d[N], r[J][N];
 #pragma unroll
-          for (int i = 0; i < V; ++i)
-            o.v[i] = kept ? (T)(w * to_f(d.v[i])) : (T)0.f;
-          store_vec(drows + (long)s * F + c, o, F - c);
+              for (int u = 0; u < N; ++u)
+                d[u] = get(dy + t * dy_pitch + at + u * step);
+              if (dw) {
+#pragma unroll
+                for (int j = 0; j < J; ++j) {
+                  const bool kept = (unsigned)s[j] < (unsigned)S;
+                  const T* src = rows + (kept ? (long)s[j] * pitch : 0) + at;
+#pragma unroll
+                  for (int u = 0; u < N; ++u) r[j][u] = get(src + u * step);
+                }
+              }
+#pragma unroll
+              for (int j = 0; j < J; ++j) {
+                if ((unsigned)s[j] >= (unsigned)M) continue;
+                const bool kept = s[j] < S;
+#pragma unroll
+                for (int u = 0; u < N; ++u) {
+                  if (dw && kept) {
+#pragma unroll
+                    for (int i = 0; i < V; ++i)
+                      dot[j] += to_f(d[u].v[i]) * to_f(r[j][u].v[i]);
+                  }
+                  if (drows) {
+                    Vec<T> o;
+#pragma unroll
+                    for (int i = 0; i < V; ++i)
+                      o.v[i] = kept ? (T)(w[j] * to_f(d[u].v[i])) : (T)0.f;
+                    put(drows + (long)s[j] * F + at + u * step, o);
+                  }
+                }
+              }
+            },
+            [&](int at) {
+              const float d = to_f(dy[t * dy_pitch + at]);
+#pragma unroll
+              for (int j = 0; j < J; ++j) {
+                if ((unsigned)s[j] >= (unsigned)M) continue;
+                const bool kept = s[j] < S;
+                if (dw && kept)
+                  dot[j] += d * to_f(rows[(long)s[j] * pitch + at]);
+                if (drows)
+                  drows[(long)s[j] * F + at] = kept ? (T)(w[j] * d) : (T)0.f;
+              }
+            });
+      if (dw) {
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+          for (int d = lanes >> 1; d > 0; d >>= 1)
+            dot[j] += __shfl_xor(dot[j], d);
+          if (in && lane == 0 && j0 + j < k) dw[t * k + j0 + j] = (W)dot[j];
         }
       }
-    }
-    if (dw) {
-      for (int d = lanes >> 1; d > 0; d >>= 1) dot += __shfl_xor(dot, d);
-      if (in && lane == 0) dw[(long)t * k + j] = (W)dot;
     }
   }
 }
@@ -491,6 +634,10 @@ int lanes_for(int F, int vec) {
     }                                                                     \
     TORCH_CHECK(false, "rows must be float32, bfloat16 or float16");      \
   }()
+
+unsigned row_blocks(long rows, int per) {
+  return (unsigned)std::min<long>((rows + per - 1) / per, 1 << 22);
+}
 
 template <typename T>
 T* ptr(const at::Tensor& t) {
@@ -531,7 +678,7 @@ at::Tensor gather_rows(const at::Tensor& x_in, const at::Tensor& offsets,
   if (out.numel() == 0) return out;
   SKA_TYPES(x.scalar_type(), [&] {
     const int lanes = lanes_for(F, Vec<T>::N), per = 256 / lanes;
-    gather_kernel<T><<<(T_rows + per - 1) / per, 256, 0, stream_now()>>>(
+    gather_kernel<T, 4><<<row_blocks(T_rows, per), 256, 0, stream_now()>>>(
         ptr<T>(x), x.stride(0), slots.data_ptr<int>(),
         offsets.data_ptr<int>() + offsets.numel() - 1, T_rows, k, F, lanes,
         ptr<T>(out));
@@ -565,18 +712,26 @@ at::Tensor combine_rows(const at::Tensor& rows_in, const at::Tensor& offsets,
   if (k == 0) return y.zero_();
   SKA_TYPES(rows.scalar_type(), [&] {
     const int lanes = lanes_for(F, Vec<T>::N), per = 256 / lanes;
-    const int blocks = (T_rows + per - 1) / per;
     const int* end = offsets.data_ptr<int>() + offsets.numel() - 1;
+    auto go = [&](auto kern, auto* w) {
+      kern<<<row_blocks(T_rows, per), 256, 0, stream_now()>>>(
+          ptr<T>(rows), rows.stride(0), slots.data_ptr<int>(), end, w, T_rows,
+          k, F, lanes, ptr<T>(y));
+      check_launch();
+    };
+    auto pick = [&](auto* w) {
+      using W = std::decay_t<decltype(*w)>;
+      if (k == 1)
+        go(combine_kernel<T, W, 1, 4>, w);
+      else if (k == 2)
+        go(combine_kernel<T, W, 2, 2>, w);
+      else
+        go(combine_kernel<T, W, 4, 2>, w);
+    };
     if (!weights || weights->dtype() == at::kFloat)
-      combine_kernel<T, float><<<blocks, 256, 0, stream_now()>>>(
-          ptr<T>(rows), rows.stride(0), slots.data_ptr<int>(), end,
-          weights ? weights->data_ptr<float>() : nullptr, T_rows, k, F, lanes,
-          ptr<T>(y));
+      pick(weights ? weights->data_ptr<float>() : (float*)nullptr);
     else
-      combine_kernel<T, T><<<blocks, 256, 0, stream_now()>>>(
-          ptr<T>(rows), rows.stride(0), slots.data_ptr<int>(), end,
-          ptr<T>(*weights), T_rows, k, F, lanes, ptr<T>(y));
-    check_launch();
+      pick(ptr<T>(*weights));
   });
   return y;
 }
@@ -613,21 +768,26 @@ combine_rows_backward(const at::Tensor& dy_in, const at::Tensor& rows_in,
   }
   SKA_TYPES(dy.scalar_type(), [&] {
     const int lanes = lanes_for(F, Vec<T>::N), per = 256 / lanes;
-    const int blocks = (T_rows + per - 1) / per;
     const int* end = offsets.data_ptr<int>() + offsets.numel() - 1;
-    T* dr = drows ? ptr<T>(*drows) : nullptr;
+    auto go = [&](auto kern, auto* w) {
+      kern<<<row_blocks(T_rows, per), 256, 0, stream_now()>>>(
+          ptr<T>(dy), dy.stride(0), ptr<T>(rows), rows.stride(0),
+          slots.data_ptr<int>(), end, w, T_rows, k, F, lanes,
+          drows ? ptr<T>(*drows) : nullptr,
+          dw ? ptr<std::decay_t<decltype(*w)>>(*dw) : nullptr);
+      check_launch();
+    };
+    auto pick = [&](auto* w) {
+      using W = std::decay_t<decltype(*w)>;
+      if (k == 1)
+        go(combine_back_kernel<T, W, 1, 2>, w);
+      else
+        go(combine_back_kernel<T, W, 2, 2>, w);
+    };
     if (!weights || weights->dtype() == at::kFloat)
-      combine_back_kernel<T, float><<<blocks, 256, 0, stream_now()>>>(
-          ptr<T>(dy), dy.stride(0), ptr<T>(rows), rows.stride(0),
-          slots.data_ptr<int>(), end,
-          weights ? weights->data_ptr<float>() : nullptr, T_rows, k, F, lanes,
-          dr, dw ? dw->data_ptr<float>() : nullptr);
+      pick(weights ? weights->data_ptr<float>() : (float*)nullptr);
     else
-      combine_back_kernel<T, T><<<blocks, 256, 0, stream_now()>>>(
-          ptr<T>(dy), dy.stride(0), ptr<T>(rows), rows.stride(0),
-          slots.data_ptr<int>(), end, ptr<T>(*weights), T_rows, k, F, lanes,
-          dr, dw ? ptr<T>(*dw) : nullptr);
-    check_launch();
+      pick(ptr<T>(*weights));
   });
   return {drows, dw};
 }
@@ -1220,12 +1380,14 @@ __global__ __launch_bounds__(256) void finish_kernel(Product p) {
   for (long e = (long)blockIdx.y * 256 + threadIdx.x; p.out && e < size;
        e += (long)gridDim.y * 256) {
     float sum = 0.f;
+#pragma unroll 8
     for (int u = 0; u < count; ++u) sum += p.part[(unit + u) * size + e];
     out[e] = (T)sum;
   }
   if (p.sums && blockIdx.y == 0)
     for (int m = threadIdx.x; m < p.M; m += 256) {
       float sum = 0.f;
+#pragma unroll 8
       for (int u = 0; u < count; ++u) sum += p.part_sums[(unit + u) * p.M + m];
       reinterpret_cast<T*>(p.sums)[(long)g * p.M + m] = (T)sum;
     }
@@ -1241,7 +1403,7 @@ __global__ __launch_bounds__(256) void finish_kernel(Product p) {
 // ---------------------------------------------------------------------------
 template <typename T>
 struct Wide {
-  typedef T Frag __attribute__((ext_vector_type(16 / sizeof(T))));
+  typedef typename Vec<T>::Values Frag;
   static __device__ __forceinline__ f32x4 go(Frag a, Frag b, f32x4 c) {
     if constexpr (sizeof(T) == 2) {
       return Mma<T>::go(a, b, c);
@@ -1253,9 +1415,7 @@ struct Wide {
     }
   }
   static __device__ __forceinline__ Frag load(const T* p) {
-    Frag v;
-    __builtin_memcpy(&v, p, 16);
-    return v;
+    return get(p).v;
   }
   static __device__ __forceinline__ Frag load(const T* p, int n) {
     Frag v;
@@ -1295,19 +1455,29 @@ __global__ __launch_bounds__(256) void narrow_kernel(Product p, bool by_row) {
              q * V;
     const int whole = p.C / kChunk * kChunk;
     int c = part * kChunk;
-#pragma unroll 4
-    for (; c < whole; c += KW * kChunk) {
-      typename Wide<T>::Frag fa[MF], fb[NF];
+    auto chunks = [&](auto n) {
+      constexpr int U = decltype(n)::value;
+      typename Wide<T>::Frag fa[U][MF], fb[U][NF];
 #pragma unroll
-      for (int i = 0; i < MF; ++i) fa[i] = Wide<T>::load(a[i] + c);
+      for (int u = 0; u < U; ++u) {
+        const int at = c + u * KW * kChunk;
 #pragma unroll
-      for (int j = 0; j < NF; ++j) fb[j] = Wide<T>::load(b[j] + c);
+        for (int i = 0; i < MF; ++i) fa[u][i] = Wide<T>::load(a[i] + at);
 #pragma unroll
-      for (int i = 0; i < MF; ++i)
+        for (int j = 0; j < NF; ++j) fb[u][j] = Wide<T>::load(b[j] + at);
+      }
 #pragma unroll
-        for (int j = 0; j < NF; ++j)
-          acc[i][j] = Wide<T>::go(fb[j], fa[i], acc[i][j]);
-    }
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int i = 0; i < MF; ++i)
+#pragma unroll
+          for (int j = 0; j < NF; ++j)
+            acc[i][j] = Wide<T>::go(fb[u][j], fa[u][i], acc[i][j]);
+    };
+    constexpr int U = MF + NF > 4 ? 2 : 4;
+    for (; c + (U - 1) * KW * kChunk < whole; c += U * KW * kChunk)
+      chunks(Count<U>{});
+    for (; c < whole; c += KW * kChunk) chunks(Count<1>{});
     if (c == whole && whole < p.C) {
       const int left = p.C - whole - q * V;
       typename Wide<T>::Frag fa[MF], fb[NF];
@@ -1530,7 +1700,7 @@ Parts take_parts(Product& p, at::TensorOptions opt) {
 template <typename T>
 void finish_launch(const Product& p) {
   const long size = (long)p.M * p.N;
-  dim3 grid(grid_of(p.G, 256), std::max(1l, std::min(1024l, size / 1024)));
+  dim3 grid(grid_of(p.G, 256), std::min(1024l, (size + 255) / 256));
   finish_kernel<T><<<grid, 256, 0, stream_now()>>>(p);
   check_launch();
 }
