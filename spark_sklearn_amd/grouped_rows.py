@@ -35,7 +35,7 @@ __all__ = ["GroupPlan", "group_rows", "gather_rows", "combine_rows",
 
 _MAX_GROUPS = (1 << 24) - 1
 _MAX_WIDTH = (1 << 21) - 1
-_functions: Any = None
+_reference: Any = None
 
 
 class GroupPlan(NamedTuple):
@@ -112,127 +112,77 @@ def _check_plan(plan, device):
 
 
 def _kernels(t):
-    """The functions that serve the tensor: native kernels on a GPU."""
+    """The functions that serve the tensor, each with its gradients: native
+    kernels on a GPU, the reference on the CPU."""
     if t.is_cuda:
         from .ops import load_extension
 
         return load_extension()
-    return _Reference
+    global _reference
+    if _reference is None:
+        _reference = _make_reference()
+    return _reference
 
 
-class _Reference:
-    @staticmethod
-    def group_rows(ids, n_groups):
-        from .models._grouped_ref import group_rows_ref
-
-        return group_rows_ref(ids, n_groups)
-
-    @staticmethod
-    def gather_rows(x, offsets, slots):
-        from .models._grouped_ref import gather_rows_ref
-
-        return gather_rows_ref(x, offsets, slots)
-
-    @staticmethod
-    def combine_rows(rows, offsets, slots, weights):
-        from .models._grouped_ref import combine_rows_ref
-
-        return combine_rows_ref(rows, offsets, slots, weights)
-
-    @staticmethod
-    def combine_rows_backward(*args):
-        from .models._grouped_ref import combine_rows_backward_ref
-
-        return combine_rows_backward_ref(*args)
-
-    @staticmethod
-    def grouped_linear(rows, weight, offsets, bias):
-        from .models._grouped_ref import grouped_linear_ref
-
-        return grouped_linear_ref(rows, weight, offsets, bias)
-
-    @staticmethod
-    def grouped_linear_drows(dy, weight, offsets):
-        from .models._grouped_ref import grouped_linear_drows_ref
-
-        return grouped_linear_drows_ref(dy, weight, offsets)
-
-    @staticmethod
-    def grouped_linear_dweight(*args):
-        from .models._grouped_ref import grouped_linear_dweight_ref
-
-        return grouped_linear_dweight_ref(*args)
-
-
-def _autograd():
-    """The autograd functions, made on first use (torch is imported late
-    throughout the package)."""
-    global _functions
-    if _functions is not None:
-        return _functions
+def _make_reference():
+    """The reference as autograd functions (torch is imported late throughout
+    the package)."""
     from types import SimpleNamespace
 
     import torch
     from torch.autograd.function import once_differentiable
 
+    from .models import _grouped_ref as ref
+
     class Gather(torch.autograd.Function):
         @staticmethod
         def forward(ctx, x, offsets, slots):
             ctx.save_for_backward(offsets, slots)
-            return _kernels(x).gather_rows(x, offsets, slots)
+            return ref.gather_rows_ref(x, offsets, slots)
 
         @staticmethod
         @once_differentiable
         def backward(ctx, grad):
-            offsets, slots = ctx.saved_tensors
             # a row's gradient is the sum over its places
-            return _kernels(grad).combine_rows(grad, offsets, slots,
-                                               None), None, None
+            return ref.combine_rows_ref(grad, *ctx.saved_tensors,
+                                        None), None, None
 
     class Combine(torch.autograd.Function):
         @staticmethod
         def forward(ctx, rows, offsets, slots, weights):
-            need_weights = ctx.needs_input_grad[3]
-            ctx.save_for_backward(rows if need_weights else None, offsets,
-                                  slots, weights)
-            return _kernels(rows).combine_rows(rows, offsets, slots, weights)
+            ctx.save_for_backward(rows, offsets, slots, weights)
+            return ref.combine_rows_ref(rows, offsets, slots, weights)
 
         @staticmethod
         @once_differentiable
         def backward(ctx, grad):
-            rows, offsets, slots, weights = ctx.saved_tensors
-            drows, dw = _kernels(grad).combine_rows_backward(
-                grad, grad if rows is None else rows, offsets, slots,
-                weights, ctx.needs_input_grad[0], ctx.needs_input_grad[3])
+            drows, dw = ref.combine_rows_backward_ref(
+                grad, *ctx.saved_tensors, ctx.needs_input_grad[0],
+                ctx.needs_input_grad[3])
             return drows, None, None, dw
 
     class Linear(torch.autograd.Function):
         @staticmethod
         def forward(ctx, rows, weight, offsets, bias):
-            need_rows, need_weight = (ctx.needs_input_grad[0],
-                                      ctx.needs_input_grad[1])
-            need_bias = ctx.needs_input_grad[3]
-            ctx.save_for_backward(rows if need_weight or need_bias else None,
-                                  weight if need_rows else None, offsets)
-            return _kernels(rows).grouped_linear(rows, weight, offsets, bias)
+            ctx.save_for_backward(rows, weight, offsets)
+            return ref.grouped_linear_ref(rows, weight, offsets, bias)
 
         @staticmethod
         @once_differentiable
         def backward(ctx, grad):
             rows, weight, offsets = ctx.saved_tensors
-            k = _kernels(grad)
-            drows = dweight = dbias = None
+            drows = None
             if ctx.needs_input_grad[0]:
-                drows = k.grouped_linear_drows(grad, weight, offsets)
-            if ctx.needs_input_grad[1] or ctx.needs_input_grad[3]:
-                dweight, dbias = k.grouped_linear_dweight(
-                    grad, rows, offsets, ctx.needs_input_grad[1],
-                    ctx.needs_input_grad[3])
+                drows = ref.grouped_linear_drows_ref(grad, weight, offsets)
+            dweight, dbias = ref.grouped_linear_dweight_ref(
+                grad, rows, offsets, ctx.needs_input_grad[1],
+                ctx.needs_input_grad[3])
             return drows, dweight, None, dbias
 
-    _functions = SimpleNamespace(Gather=Gather, Combine=Combine,
-                                 Linear=Linear)
-    return _functions
+    return SimpleNamespace(
+        group_rows=ref.group_rows_ref, gather_rows=Gather.apply,
+        combine_rows=Combine.apply, grouped_linear=Linear.apply,
+        grouped_linear_dweight=ref.grouped_linear_dweight_ref)
 
 
 def group_rows(ids, n_groups: int) -> GroupPlan:
@@ -276,7 +226,7 @@ def gather_rows(x, plan: GroupPlan):
     offsets, slots = _check_plan(plan, x.device)
     _require(slots.shape[0] == x.shape[0], ValueError,
              f"x has {x.shape[0]} rows, the plan {slots.shape[0]}")
-    return _autograd().Gather.apply(x, offsets, slots)
+    return _kernels(x).gather_rows(x, offsets, slots)
 
 
 def combine_rows(rows, plan: GroupPlan, weights=None):
@@ -308,7 +258,7 @@ def combine_rows(rows, plan: GroupPlan, weights=None):
                  f"weights must have the ids' shape "
                  f"{tuple(plan.slots.shape)}, got {tuple(weights.shape)}")
         weights = weights.reshape(slots.shape).contiguous()
-    return _autograd().Combine.apply(rows, offsets, slots, weights)
+    return _kernels(rows).combine_rows(rows, offsets, slots, weights)
 
 
 def grouped_linear(rows, weight, offsets, bias: Optional[Any] = None):
@@ -356,5 +306,5 @@ def grouped_linear(rows, weight, offsets, bias: Optional[Any] = None):
         _require(tuple(bias.shape) == (G, N), ValueError,
                  f"bias must be {(G, N)}, got {tuple(bias.shape)}")
         bias = bias.contiguous()
-    return _autograd().Linear.apply(rows, weight.contiguous(),
-                                    offsets.contiguous(), bias)
+    return _kernels(rows).grouped_linear(rows, weight.contiguous(),
+                                         offsets.contiguous(), bias)

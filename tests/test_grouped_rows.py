@@ -401,6 +401,19 @@ def test_gradcheck_reference():
         whole, [v.requires_grad_() for v in (x, weight, bias, w)])
 
 
+@pytest.mark.parametrize("device", DEVICES)
+def test_differentiates_once_only(device):
+    """A second differentiation is an error, never a silent zero."""
+    x, ids, weight, bias, w, dy = chain_data(device, T=20)
+    for i in range(4):
+        leaves = [v.detach().requires_grad_(j == i)
+                  for j, v in enumerate((x, weight, bias, w))]
+        y = chain(leaves[0], ids, weight.shape[0], *leaves[1:])
+        g, = torch.autograd.grad((y * y).sum(), leaves[i], create_graph=True)
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(g.sum(), leaves[i])
+
+
 def chain(x, ids, G, weight, bias, w):
     plan = ska.group_rows(ids, G)
     rows = ska.gather_rows(x, plan)
