@@ -1036,18 +1036,33 @@ struct Mma<_Float16> {
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
 #define SKA_LDS(T, p) ((__attribute__((address_space(3))) T*)(p))
 
-// One operand's tile of EXT rows (m or n) by kStep steps of c.
-template <typename T, int EXT, bool ACROSS, int THREADS>
+// One operand's tile of EXT rows (m or n) by kStep steps of c.  With FRAGS > 1
+// the rows of FRAGS neighbouring fragments are dealt out 4 at a time: row r of
+// fragment j is (r / 4) * 4 * FRAGS + j * 4 + r % 4 of their 16 * FRAGS.  A
+// lane of the product then holds 4 * FRAGS neighbouring n.
+template <typename T, int EXT, bool ACROSS, int THREADS, int FRAGS>
 struct Tile {
   static constexpr int kGranules = EXT * kStep / 8;
   static constexpr int kPer = kGranules / THREADS;
   static constexpr int kAcross = EXT / 8;  // granules of one step of c
   static constexpr int kBytes = EXT * kStep * 2;
 
+  // how the granules of an along row, or of an across step, are moved, so
+  // that the 8 rows of 8 lanes (the 4 steps of 16) lie in different banks
+  static __device__ __forceinline__ int swap(int row) {
+    return FRAGS == 1   ? row & 7
+           : FRAGS == 2 ? (row & 3) | ((row >> 1) & 4)
+                        : (row & 3) | ((row >> 2) & 4);
+  }
   static __device__ __forceinline__ int move(int c) {
-    return (((c & 3) << 1) | (((c >> 3) & 1) << 3)) & (kAcross - 1);
+    if (FRAGS == 1)
+      return (((c & 3) << 1) | (((c >> 3) & 1) << 3)) & (kAcross - 1);
+    if (FRAGS == 2)
+      return ((c & 1) | ((c & 2) << 1) | ((c & 8) >> 0)) & (kAcross - 1);
+    return ((c & 1) | ((c & 2) << 2)) & (kAcross - 1);
   }
   // the first row and step of the granule at LDS place g
   static __device__ __forceinline__ void place(int g, int& row, int& c) {
@@ -1056,77 +1071,85 @@ struct Tile {
       row = ((g % kAcross) ^ move(c)) * 8;
     } else {
       row = g >> 3;
-      c = ((g & 7) ^ (row & 7)) * 8;
+      c = ((g & 7) ^ swap(row)) * 8;
     }
-  }
-  // Which part of a granule may be read: 8 for all of it.  `room` is the
-  // number of values from `src` to the end of the matrix: an across granule
-  // may run into the next row, whose values meet outputs that are not stored.
-  static __device__ __forceinline__ int part(int row, int c, long pitch,
-                                             int rows, int steps, long room) {
-    if (row >= rows || c >= steps) return 0;
-    if (ACROSS) {
-      const int n = rows - row;
-      return n >= 8 || c * pitch + row + 8 <= room ? 8 : n;
-    }
-    return min(8, steps - c);
   }
   static __device__ __forceinline__ long at(int row, int c, long pitch) {
     return ACROSS ? c * pitch + row : row * pitch + c;
   }
-  // whether any granule is read in part
-  static __device__ __forceinline__ bool ragged(long pitch, int rows,
-                                                int steps, long room) {
-    if (ACROSS)
-      return (rows & 7) &&
-             (min(steps, kStep) - 1) * pitch + ((rows + 7) & ~7) > room;
-    return steps < kStep && (steps & 7);
+  // Granules are read whole below these bounds.  An across granule at the
+  // edge may run into the next row, whose values meet outputs that are not
+  // stored, unless it would leave the matrix: `room` is the number of values
+  // from `src` to the matrix's end.
+  struct Bounds {
+    int rows, steps;
+    bool ragged;  // some granules are left to fill()
+  };
+  static __device__ __forceinline__ Bounds bounds(long pitch, int rows,
+                                                  int steps, long room) {
+    if (ACROSS) {
+      const bool cut = (rows & 7) && (min(steps, kStep) - 1) * pitch +
+                                             ((rows + 7) & ~7) >
+                                         room;
+      return {cut ? rows & ~7 : rows, steps, cut};
+    }
+    return {rows, steps & ~7, steps < kStep && (steps & 7)};
   }
+  // Written in assembly, because the compiler would wait for all loads under
+  // way before it reads LDS; whoever reads the tile waits with wait_loads.
   static __device__ __forceinline__ void load_async(const T* src, long pitch,
-                                                    int rows, int steps,
-                                                    long room, char* lds) {
+                                                    Bounds b, char* lds) {
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(
-        (void*)src, 0, 0x7fffffff, 0x00020000);
+    const unsigned long base = reinterpret_cast<unsigned long>(src);
+    // base, no stride, 2^31 - 1 bytes, raw
+    const i32x4 rsrc = {(int)base, (int)(base >> 32) & 0xffff, 0x7fffffff,
+                        0x00020000};
+    const unsigned to = __builtin_amdgcn_readfirstlane(
+        (unsigned)(uintptr_t)SKA_LDS(void, lds) + wave * 1024);
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-      const int g0 = i * THREADS + wave * 64;
       int row, c;
-      place(g0 + lane, row, c);
-      const bool in = part(row, c, pitch, rows, steps, room) == 8;
+      place(i * THREADS + wave * 64 + lane, row, c);
+      const bool in = row < b.rows && c < b.steps;
       const unsigned off = in ? (unsigned)at(row, c, pitch) * 2 : 0x80000000u;
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(
-          rsrc, SKA_LDS(void, lds + g0 * 16), 16, off, 0, 0, 0);
+      asm volatile(
+          "s_mov_b32 m0, %0\n\t"
+          "s_nop 0\n\t"
+          "buffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(to + i * THREADS * 16),
+          "v"(off), "s"(rsrc)
+          : "memory", "m0");
     }
   }
-  // after the loads above have ended: the granules that were left out
+  // The granules that load_async left out, after its loads have ended.
   static __device__ __forceinline__ void fill(const T* src, long pitch,
-                                              int rows, int steps, long room,
+                                              int rows, int steps, Bounds b,
                                               char* lds) {
 #pragma unroll 1
     for (int i = 0; i < kPer; ++i) {
       const int g = i * THREADS + threadIdx.x;
       int row, c;
       place(g, row, c);
-      const int n = part(row, c, pitch, rows, steps, room);
-      if (n == 0 || n == 8) continue;
+      const int n = ACROSS ? (row >= b.rows && c < steps ? rows - row : 0)
+                           : (c >= b.steps && row < rows ? steps - c : 0);
       T* to = reinterpret_cast<T*>(lds + g * 16);
       const T* from = src + at(row, c, pitch);
-      for (int e = 0; e < n; ++e) to[e] = from[e];
+      for (int e = 0; e < min(n, 8); ++e) to[e] = from[e];
     }
   }
   // rows that begin at odd addresses: through registers
   static __device__ __forceinline__ void load_regs(const T* src, long pitch,
                                                    int rows, int steps,
-                                                   long room,
+                                                   Bounds b,
                                                    Vec<T> (&v)[kPer]) {
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
       int row, c;
       place(i * THREADS + threadIdx.x, row, c);
-      const int n = part(row, c, pitch, rows, steps, room);
-      v[i] = load_vec(src + (n ? at(row, c, pitch) : 0), n);
+      int n = row < b.rows && c < b.steps ? 8 : 0;
+      if (b.ragged && n == 0 && row < rows && c < steps)
+        n = ACROSS ? rows - row : steps - c;
+      v[i] = load_vec(src + (n > 0 ? at(row, c, pitch) : 0), n);
     }
   }
   static __device__ __forceinline__ void store_regs(const Vec<T> (&v)[kPer],
@@ -1136,29 +1159,58 @@ struct Tile {
       *reinterpret_cast<Vec<T>*>(lds + (i * THREADS + threadIdx.x) * 16) =
           v[i];
   }
-  // the fragment of rows [row0, row0 + 16) and steps [c0, c0 + 32)
+  // fragment j of the rows from row0 and the steps [c0, c0 + 32)
   static __device__ __forceinline__ typename Mma<T>::Frag frag(
-      const char* lds, int row0, int c0) {
+      const char* lds, int row0, int j, int c0) {
     const int lane = threadIdx.x & 63;
     const int r = lane & 15, q = lane >> 4;
     if (ACROSS) {
+      // lane (4 * step + s) of 16 reads rows 4 * s .. 4 * s + 3 of the fragment
+      const int row = row0 + (FRAGS == 1 ? j * 16 + (r & 3) * 4
+                                         : (r & 3) * 4 * FRAGS + j * 4);
       s16x4 v[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int c = c0 + q * 8 + h * 4 + (r >> 2);
-        const int g = ((row0 >> 3) + ((r & 3) >> 1)) ^ move(c);
+        const int g = (row >> 3) ^ move(c);
         v[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            SKA_LDS(s16x4, lds + (c * kAcross + g) * 16 + (r & 1) * 8));
+            SKA_LDS(s16x4, lds + (c * kAcross + g) * 16 + (row & 4) * 2));
       }
       const s16x8 w = {v[0][0], v[0][1], v[0][2], v[0][3],
                        v[1][0], v[1][1], v[1][2], v[1][3]};
       return __builtin_bit_cast(typename Mma<T>::Frag, w);
     }
-    const int row = row0 + r;
+    const int row = row0 + (FRAGS == 1 ? j * 16 + r
+                                       : (r >> 2) * 4 * FRAGS + j * 4 +
+                                             (r & 3));
     return *reinterpret_cast<const typename Mma<T>::Frag*>(
-        lds + (row * 8 + (((c0 >> 3) + q) ^ (row & 7))) * 16);
+        lds + (row * 8 + (((c0 >> 3) + q) ^ swap(row))) * 16);
   }
 };
+
+// Waits until at most `later` tiles of N loads each are under way.
+template <int N, int MOST>
+__device__ __forceinline__ void wait_loads(int later) {
+  if constexpr (MOST > 0) {
+    if (later >= MOST) {
+      // vmcnt(N * MOST), nothing else
+      __builtin_amdgcn_s_waitcnt(0x0f70 | ((N * MOST) & 15) |
+                                 (((N * MOST) >> 4) << 14));
+      return;
+    }
+    wait_loads<N, MOST - 1>(later);
+  } else {
+    __builtin_amdgcn_s_waitcnt(0x0f70);
+  }
+}
+
+// A barrier for what the block wrote to LDS itself; loads under way go on.
+__device__ __forceinline__ void block_barrier() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
 
 struct Product {
   const void* a;
@@ -1177,13 +1229,15 @@ struct Product {
   float* part_sums;
 };
 
-template <typename T, int BM, int BN, int WM, int WN, int MODE, bool ASYNC>
+template <typename T, int BM, int BN, int WM, int WN, int MODE, int STAGES>
 __global__ __launch_bounds__(WM* WN * 64) void product_kernel(Product p) {
   constexpr int kThreads = WM * WN * 64;
   constexpr int FM = BM / WM / 16, FN = BN / WN / 16;
-  typedef Tile<T, BM, MODE == kDWeight, kThreads> TA;
-  typedef Tile<T, BN, MODE != kForward, kThreads> TB;
-  __shared__ __align__(16) char lds[2][TA::kBytes + TB::kBytes];
+  typedef Tile<T, BM, MODE == kDWeight, kThreads, 1> TA;
+  typedef Tile<T, BN, MODE != kForward, kThreads, FN> TB;
+  constexpr bool ASYNC = STAGES > 0;
+  constexpr int kBuffers = ASYNC ? STAGES : 2;
+  __shared__ __align__(16) char lds[kBuffers][TA::kBytes + TB::kBytes];
 
   // Blocks go round the 8 XCDs: each gets a contiguous run of tiles, whose
   // operands its L2 then holds.
@@ -1259,97 +1313,117 @@ __global__ __launch_bounds__(WM* WN * 64) void product_kernel(Product p) {
   for (int i = 0; i < 8; ++i) ones[i] = (T)1.f;
 
   Vec<T> ra[ASYNC ? 1 : TA::kPer], rb[ASYNC ? 1 : TB::kPer];
+  // The tile's place at step c, and which of its granules are whole.
+  auto source = [&](int c, const T*& a, const T*& b,
+                    typename TA::Bounds& ba, typename TB::Bounds& bb) {
+    const long at = c / kStep;
+    a = A + at * a_step;
+    b = B + at * b_step;
+    ba = TA::bounds(p.a_pitch, rows, steps - c, a_room - at * a_step);
+    bb = TB::bounds(p.b_pitch, cols, steps - c, b_room - at * b_step);
+  };
   auto load = [&](int c, int buf) {
-    const long left = (long)(c / kStep);
-    const T* a = A + left * a_step;
-    const T* b = B + left * b_step;
+    const T *a, *b;
+    typename TA::Bounds ba;
+    typename TB::Bounds bb;
+    source(c, a, b, ba, bb);
     if constexpr (ASYNC) {
-      TA::load_async(a, p.a_pitch, rows, steps - c, a_room - left * a_step,
-                     lds[buf]);
-      TB::load_async(b, p.b_pitch, cols, steps - c, b_room - left * b_step,
-                     lds[buf] + TA::kBytes);
+      TA::load_async(a, p.a_pitch, ba, lds[buf]);
+      TB::load_async(b, p.b_pitch, bb, lds[buf] + TA::kBytes);
     } else {
-      TA::load_regs(a, p.a_pitch, rows, steps - c, a_room - left * a_step,
-                    ra);
-      TB::load_regs(b, p.b_pitch, cols, steps - c, b_room - left * b_step,
-                    rb);
+      TA::load_regs(a, p.a_pitch, rows, steps - c, ba, ra);
+      TB::load_regs(b, p.b_pitch, cols, steps - c, bb, rb);
     }
   };
-  auto land = [&](int c, int buf) {
+  // Ends the loads of the tile at c: all but those of the `later` tiles that
+  // were issued behind them.
+  constexpr int kLoads = TA::kPer + TB::kPer;
+  auto land = [&](int c, int buf, int later) {
     if constexpr (ASYNC) {
-      __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
-      const long left = (long)(c / kStep);
-      const long ar = a_room - left * a_step, br = b_room - left * b_step;
-      if (TA::ragged(p.a_pitch, rows, steps - c, ar))
-        TA::fill(A + left * a_step, p.a_pitch, rows, steps - c, ar, lds[buf]);
-      if (TB::ragged(p.b_pitch, cols, steps - c, br))
-        TB::fill(B + left * b_step, p.b_pitch, cols, steps - c, br,
-                 lds[buf] + TA::kBytes);
+      wait_loads<kLoads, STAGES - 2>(later);
+      const T *a, *b;
+      typename TA::Bounds ba;
+      typename TB::Bounds bb;
+      source(c, a, b, ba, bb);
+      if (ba.ragged) TA::fill(a, p.a_pitch, rows, steps - c, ba, lds[buf]);
+      if (bb.ragged)
+        TB::fill(b, p.b_pitch, cols, steps - c, bb, lds[buf] + TA::kBytes);
     } else {
       TA::store_regs(ra, lds[buf]);
       TB::store_regs(rb, lds[buf] + TA::kBytes);
     }
+    block_barrier();
   };
 
-  if (steps > 0) load(0, 0);
-  for (int c = 0, buf = 0; c < steps; c += kStep, buf ^= 1) {
-    land(c, buf);
-    __syncthreads();
-    if (c + kStep < steps) load(c + kStep, buf ^ 1);
+  constexpr int kAhead = ASYNC ? STAGES - 1 : 1;
+#pragma unroll
+  for (int s = 0; s < kAhead; ++s)
+    if (s * kStep < steps) load(s * kStep, s);
+  int buf = 0;
+  for (int c = 0; c < steps; c += kStep) {
+    const int later =
+        min(kAhead - 1, (steps - c - 1) / kStep);  // tiles behind this one
+    land(c, buf, later);
+    const int far = c + kAhead * kStep;
+    if (far < steps) load(far, (buf + kAhead) % kBuffers);
     const char* la = lds[buf];
     const char* lb = lds[buf] + TA::kBytes;
 #pragma unroll
     for (int h = 0; h < kStep; h += 32) {
       typename Mma<T>::Frag fb[FN];
 #pragma unroll
-      for (int j = 0; j < FN; ++j) fb[j] = TB::frag(lb, wn + j * 16, h);
+      for (int j = 0; j < FN; ++j) fb[j] = TB::frag(lb, wn, j, h);
 #pragma unroll
       for (int i = 0; i < FM; ++i) {
-        const typename Mma<T>::Frag fa = TA::frag(la, wm + i * 16, h);
+        const typename Mma<T>::Frag fa = TA::frag(la, wm, i, h);
 #pragma unroll
         for (int j = 0; j < FN; ++j)
           acc[i][j] = Mma<T>::go(fb[j], fa, acc[i][j]);
         if (MODE == kDWeight && sums) sum[i] = Mma<T>::go(ones, fa, sum[i]);
       }
     }
+    buf = buf + 1 == kBuffers ? 0 : buf + 1;
   }
 
-  // lane: row m = lane & 15 of its tile, 4 columns from (lane >> 4) * 4
+  // lane: row m = lane & 15 of each fragment, 4 * FN neighbouring columns
   T* out = reinterpret_cast<T*>(p.out);
   const T* bias = reinterpret_cast<const T*>(p.bias);
-#pragma unroll
-  for (int j = 0; j < FN; ++j) {
-    const int n = wn + j * 16 + (lane >> 4) * 4;
-    if (n >= cols) continue;
-    const int left = cols - n;
-    float add[4] = {};
+  const int n = wn + (lane >> 4) * 4 * FN;
+  const int left = cols - n;
+  if (left > 0 && (MODE != kDWeight || out)) {
+    float add[FN][4] = {};
     if (MODE == kForward && bias && group < p.G) {
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
-        if (r < left) add[r] = to_f(bias[(long)group * p.N + n0 + n + r]);
+      for (int j = 0; j < FN * 4; ++j)
+        if (j < left)
+          add[j >> 2][j & 3] = to_f(bias[(long)group * p.N + n0 + n + j]);
     }
 #pragma unroll
     for (int i = 0; i < FM; ++i) {
       const int m = wm + i * 16 + (lane & 15);
       if (m >= rows) continue;
-      T v[4];
+      const long at = (out_row + m) * p.N + n0 + n;
+      if (MODE == kDWeight && parted) {
 #pragma unroll
-      for (int r = 0; r < 4; ++r) v[r] = (T)(acc[i][j][r] + add[r]);
-      if (MODE == kDWeight && out && parted) {
-        float* to = p.part + (out_row + m) * p.N + n0 + n;
-        if (left >= 4) {
-          __builtin_memcpy(to, &acc[i][j], 16);
-        } else {
-          for (int r = 0; r < left; ++r) to[r] = acc[i][j][r];
+        for (int j = 0; j < FN; ++j) {
+          if (left >= j * 4 + 4) {
+            *reinterpret_cast<Bytes16*>(p.part + at + j * 4) =
+                __builtin_bit_cast(Bytes16, acc[i][j]);
+          } else {
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (j * 4 + r < left) p.part[at + j * 4 + r] = acc[i][j][r];
+          }
         }
         continue;
       }
-      if (MODE == kDWeight && !out) continue;
-      T* to = out + (out_row + m) * p.N + n0 + n;
-      if (left >= 4) {
-        __builtin_memcpy(to, v, 8);
-      } else {
-        for (int r = 0; r < left; ++r) to[r] = v[r];
+#pragma unroll
+      for (int j = 0; j < FN; j += 2) {
+        Vec<T> v;
+#pragma unroll
+        for (int r = 0; r < 8; ++r)
+          v.v[r] = (T)(acc[i][j + r / 4][r & 3] + add[j + r / 4][r & 3]);
+        store_vec(out + at + j * 4, v, left - j * 4);
       }
     }
   }
@@ -1713,29 +1787,71 @@ void product_launch(Product p, at::TensorOptions opt) {
                      whole_words((const T*)p.b, p.b_pitch) &&
                      // the weights of a group may begin at an odd value
                      (MODE == kDWeight || ((long)p.N * p.C) % 2 == 0);
+  auto tiles = [&](long b) { return (p.M + b - 1) / b * ((p.N + b - 1) / b); };
   auto go = [&](auto kern, int bm, int bn, int threads) {
-    const long m_tiles = (p.M + bm - 1) / bm, n_tiles = (p.N + bn - 1) / bn;
+    const long m_tiles = (p.M + bm - 1) / bm;
     long mt = (long)p.M / bm + p.G + 1;
     Parts parts;
     if (MODE == kDWeight) {
       mt = p.G * m_tiles;
-      if (mt * n_tiles < 512) {
-        p.shift = part_shift(p.C, m_tiles * n_tiles, 512);
+      const long all = m_tiles * ((p.N + bn - 1) / bn);
+      if (bm == 64 && all * p.G < 512) {
+        p.shift = part_shift(p.C, all, 512);
         parts = take_parts(p, opt);
         mt = ((p.C >> p.shift) + p.G + 1) * m_tiles;
       }
     }
-    const long nt = p.out ? n_tiles : 1;
+    const long nt = p.out ? (p.N + bn - 1) / bn : 1;
     kern<<<grid_of(mt * nt, threads), threads, 0, stream_now()>>>(p);
     check_launch();
     if (MODE == kDWeight && p.shift) finish_launch<T>(p);
   };
-  if (!async)
-    go(product_kernel<T, 128, 128, 2, 2, MODE, false>, 128, 128, 256);
-  else if (p.M <= 128 || p.N <= 128)
-    go(product_kernel<T, 128, 128, 2, 2, MODE, true>, 128, 128, 256);
+  // Larger tiles read less and fill the matrix units better; smaller ones
+  // waste less of the groups' last tiles and leave more blocks to hide the
+  // loads behind.  Measured on bfloat16, us for 256^2 / 128^2 / 64 x 128 /
+  // 64^2 tiles (rows, groups, outputs, columns):
+  //   forward  65536, 32, 4096, 1024:  685 / 788 / 1178 / 1195
+  //            16384, 64, 1024, 1024:   64 /  57 /   68 /   75
+  //             8198, 48,  768,  768:   28 /  28 /   24 /   26
+  //             8192,  8,  256,  256:   12 /   7 /    7 /    6
+  //   dweight  65536, 32, 4096, 1024:  747 / 931 / 1511 / 1447
+  //             8198, 48,  768,  768:   36 /  33 /   49 /   47
+  //            65536, 256,  64,  256:   46 /  34 /   31 /   24
+  if (MODE == kDWeight) {
+    // 256^2 where that fills the card and its edges waste less than a third
+    const bool large = p.G * tiles(256) >= 192 &&
+                       tiles(256) * 65536 * 3 <= 4l * p.M * p.N;
+    const bool middle = p.M > 64 && p.N > 64 && p.G * tiles(128) >= 256;
+    if (async && large)
+      go(product_kernel<T, 256, 256, 2, 4, MODE, 2>, 256, 256, 512);
+    else if (async && middle)
+      go(product_kernel<T, 128, 128, 2, 2, MODE, 2>, 128, 128, 256);
+    else if (async)
+      go(product_kernel<T, 64, 64, 2, 2, MODE, 3>, 64, 64, 256);
+    else if (large || middle)
+      go(product_kernel<T, 128, 128, 2, 2, MODE, 0>, 128, 128, 256);
+    else
+      go(product_kernel<T, 64, 64, 2, 2, MODE, 0>, 64, 64, 256);
+    return;
+  }
+  const long each = p.M / std::min(p.G, p.M);  // rows a group
+  auto row_tiles = [&](long bm, long bn) {
+    return (p.M / bm + std::min(p.G, p.M) / 2 + 1) * ((p.N + bn - 1) / bn);
+  };
+  const bool large = each >= 768 && p.N > 128 && row_tiles(256, 256) >= 512;
+  const bool middle = each >= 192 && p.N > 64 && row_tiles(128, 128) >= 256;
+  if (async && large)
+    go(product_kernel<T, 256, 256, 2, 4, MODE, 2>, 256, 256, 512);
+  else if (async && middle)
+    go(product_kernel<T, 128, 128, 2, 2, MODE, 2>, 128, 128, 256);
+  else if (async && p.N > 64 && row_tiles(64, 128) >= 256)
+    go(product_kernel<T, 64, 128, 1, 4, MODE, 3>, 64, 128, 256);
+  else if (async)
+    go(product_kernel<T, 64, 64, 2, 2, MODE, 3>, 64, 64, 256);
+  else if (large || middle)
+    go(product_kernel<T, 128, 128, 2, 2, MODE, 0>, 128, 128, 256);
   else
-    go(product_kernel<T, 256, 256, 2, 4, MODE, true>, 256, 256, 512);
+    go(product_kernel<T, 64, 64, 2, 2, MODE, 0>, 64, 64, 256);
 }
 
 void narrow_dweight_launch(Product p, at::TensorOptions opt) {
