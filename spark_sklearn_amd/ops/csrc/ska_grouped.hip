@@ -648,8 +648,11 @@ T* ptr(const at::Tensor& t) {
 // A matrix whose rows may lie apart but are contiguous in themselves.
 at::Tensor packed_rows(const at::Tensor& t) {
   if (t.size(0) == 0 || t.size(1) == 0) return t;
-  const bool fits = (t.size(1) == 1 || t.stride(1) == 1) &&
-                    (t.size(0) == 1 || t.stride(0) >= t.size(1));
+  // the product kernels' offsets in a tile of 256 rows pass no 31 bits
+  const bool fits =
+      (t.size(1) == 1 || t.stride(1) == 1) &&
+      (t.size(0) == 1 ||
+       (t.stride(0) >= t.size(1) && t.stride(0) < (1 << 22)));
   return fits ? t : t.contiguous();
 }
 
@@ -1014,7 +1017,6 @@ __global__ __launch_bounds__(256) void weights_plain_kernel(
 // The matrix instruction gets B first: a lane then holds 4 neighbouring n of
 // one m, and stores them together.
 // ---------------------------------------------------------------------------
-constexpr int kStep = 64;
 enum Mode { kForward, kDRows, kDWeight };
 
 template <typename T>
@@ -1039,23 +1041,24 @@ typedef short s16x8 __attribute__((ext_vector_type(8)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 #define SKA_LDS(T, p) ((__attribute__((address_space(3))) T*)(p))
 
-// One operand's tile of EXT rows (m or n) by kStep steps of c.  With FRAGS > 1
+// One operand's tile of EXT rows (m or n) by KS steps of c.  With FRAGS > 1
 // the rows of FRAGS neighbouring fragments are dealt out 4 at a time: row r of
 // fragment j is (r / 4) * 4 * FRAGS + j * 4 + r % 4 of their 16 * FRAGS.  A
 // lane of the product then holds 4 * FRAGS neighbouring n.
-template <typename T, int EXT, bool ACROSS, int THREADS, int FRAGS>
+template <typename T, int EXT, int KS, bool ACROSS, int THREADS, int FRAGS>
 struct Tile {
-  static constexpr int kGranules = EXT * kStep / 8;
+  static constexpr int kGranules = EXT * KS / 8;
   static constexpr int kPer = kGranules / THREADS;
   static constexpr int kAcross = EXT / 8;  // granules of one step of c
-  static constexpr int kBytes = EXT * kStep * 2;
+  static constexpr int kBytes = EXT * KS * 2;
 
   // how the granules of an along row, or of an across step, are moved, so
   // that the 8 rows of 8 lanes (the 4 steps of 16) lie in different banks
+  static constexpr int kAlong = KS / 8;  // granules of one along row
   static __device__ __forceinline__ int swap(int row) {
-    return FRAGS == 1   ? row & 7
-           : FRAGS == 2 ? (row & 3) | ((row >> 1) & 4)
-                        : (row & 3) | ((row >> 2) & 4);
+    const int high = FRAGS == 1 ? row >> 2 : FRAGS == 2 ? row >> 3 : row >> 4;
+    if (KS == 32) return ((row >> 1) & 1) | (high & 1) << 1;
+    return (row & 3) | (high & 1) << 2;
   }
   static __device__ __forceinline__ int move(int c) {
     if (FRAGS == 1)
@@ -1070,8 +1073,8 @@ struct Tile {
       c = g / kAcross;
       row = ((g % kAcross) ^ move(c)) * 8;
     } else {
-      row = g >> 3;
-      c = ((g & 7) ^ swap(row)) * 8;
+      row = g / kAlong;
+      c = ((g % kAlong) ^ swap(row)) * 8;
     }
   }
   static __device__ __forceinline__ long at(int row, int c, long pitch) {
@@ -1088,17 +1091,19 @@ struct Tile {
   static __device__ __forceinline__ Bounds bounds(long pitch, int rows,
                                                   int steps, long room) {
     if (ACROSS) {
-      const bool cut = (rows & 7) && (min(steps, kStep) - 1) * pitch +
+      const bool cut = (rows & 7) && (min(steps, KS) - 1) * pitch +
                                              ((rows + 7) & ~7) >
                                          room;
       return {cut ? rows & ~7 : rows, steps, cut};
     }
-    return {rows, steps & ~7, steps < kStep && (steps & 7)};
+    return {rows, steps & ~7, steps < KS && (steps & 7)};
   }
-  // Written in assembly, because the compiler would wait for all loads under
-  // way before it reads LDS; whoever reads the tile waits with wait_loads.
+  // One of a wave's kPer loads.  Written in assembly, because the compiler
+  // would wait for all loads under way before it reads LDS; whoever reads the
+  // tile waits for them itself.
   static __device__ __forceinline__ void load_async(const T* src, long pitch,
-                                                    Bounds b, char* lds) {
+                                                    Bounds b, char* lds,
+                                                    int i) {
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const unsigned long base = reinterpret_cast<unsigned long>(src);
@@ -1107,21 +1112,18 @@ struct Tile {
                         0x00020000};
     const unsigned to = __builtin_amdgcn_readfirstlane(
         (unsigned)(uintptr_t)SKA_LDS(void, lds) + wave * 1024);
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      int row, c;
-      place(i * THREADS + wave * 64 + lane, row, c);
-      const bool in = row < b.rows && c < b.steps;
-      const unsigned off = in ? (unsigned)at(row, c, pitch) * 2 : 0x80000000u;
-      asm volatile(
-          "s_mov_b32 m0, %0\n\t"
-          "s_nop 0\n\t"
-          "buffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(to + i * THREADS * 16),
-          "v"(off), "s"(rsrc)
-          : "memory", "m0");
-    }
+    int row, c;
+    place(i * THREADS + wave * 64 + lane, row, c);
+    const bool in = row < b.rows && c < b.steps;
+    const unsigned off = in ? (unsigned)at(row, c, pitch) * 2 : 0x80000000u;
+    asm volatile(
+        "s_mov_b32 m0, %0\n\t"
+        "s_nop 0\n\t"
+        "buffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(to + i * THREADS * 16),
+        "v"(off), "s"(rsrc)
+        : "memory", "m0");
   }
-  // The granules that load_async left out, after its loads have ended.
+  // The granules that load_async leaves out, after its loads have ended.
   static __device__ __forceinline__ void fill(const T* src, long pitch,
                                               int rows, int steps, Bounds b,
                                               char* lds) {
@@ -1184,24 +1186,14 @@ struct Tile {
                                        : (r >> 2) * 4 * FRAGS + j * 4 +
                                              (r & 3));
     return *reinterpret_cast<const typename Mma<T>::Frag*>(
-        lds + (row * 8 + (((c0 >> 3) + q) ^ swap(row))) * 16);
+        lds + (row * kAlong + (((c0 >> 3) + q) ^ swap(row))) * 16);
   }
 };
 
-// Waits until at most `later` tiles of N loads each are under way.
-template <int N, int MOST>
-__device__ __forceinline__ void wait_loads(int later) {
-  if constexpr (MOST > 0) {
-    if (later >= MOST) {
-      // vmcnt(N * MOST), nothing else
-      __builtin_amdgcn_s_waitcnt(0x0f70 | ((N * MOST) & 15) |
-                                 (((N * MOST) >> 4) << 14));
-      return;
-    }
-    wait_loads<N, MOST - 1>(later);
-  } else {
-    __builtin_amdgcn_s_waitcnt(0x0f70);
-  }
+// Waits until at most N loads are under way.
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+  __builtin_amdgcn_s_waitcnt(0x0f70 | (N & 15) | ((N >> 4) << 14));
 }
 
 // A barrier for what the block wrote to LDS itself; loads under way go on.
@@ -1227,183 +1219,245 @@ struct Product {
   int shift;
   float* part;
   float* part_sums;
+  int tiles;  // output tiles of the launch
 };
 
+// One tile of the output: its operands and where it goes.
+template <typename T>
+struct Job {
+  const T *a, *b;
+  long a_room, b_room, out_row;
+  int group, rows, cols, n0;
+  int steps;  // of c; 0: an output of zeros
+  bool parted;
+};
+
+// Tile number `tile` of the launch, if there is such a one.
+template <typename T, int BM, int BN, int MODE>
+__device__ __forceinline__ bool find_job(const Product& p, int tile,
+                                         Job<T>& job) {
+  const int nt = p.out ? (p.N + BN - 1) / BN : 1;
+  const int mt = p.tiles / nt;
+  const T* A = reinterpret_cast<const T*>(p.a);
+  const T* B = reinterpret_cast<const T*>(p.b);
+  if (MODE == kDWeight) {
+    job.n0 = (tile % nt) * BN;
+    tile /= nt;
+    const int each = (p.M + BM - 1) / BM;
+    const int unit = tile / each;
+    const int m0 = (tile % each) * BM;
+    int first, start = 0;
+    job.parted = false;
+    if (p.shift) {
+      const Segment seg = find_segment(p.offsets, p.G, p.C, unit, p.shift);
+      if (seg.first >= seg.end || seg.group >= p.G) return false;
+      job.group = seg.group;
+      first = seg.first;
+      start = seg.start;
+      job.steps = min(seg.end - first, 1 << p.shift);
+      job.parted = seg.end - seg.start > (1 << p.shift);
+    } else {
+      job.group = unit;
+      first = __builtin_amdgcn_readfirstlane(edge(p.offsets, unit, p.G, p.C));
+      job.steps = __builtin_amdgcn_readfirstlane(
+                      edge(p.offsets, unit + 1, p.G, p.C)) -
+                  first;
+    }
+    job.rows = min(BM, p.M - m0);
+    job.out_row = (job.parted ? part_place(start, p.shift) +
+                                    ((first - start) >> p.shift)
+                              : (long)job.group) *
+                      p.M +
+                  m0;
+    job.a = A + first * p.a_pitch + m0;
+    job.b = B + first * p.b_pitch + job.n0;
+    job.a_room = (long)(p.C - first - 1) * p.a_pitch + p.M - m0;
+    job.b_room = (long)(p.C - first - 1) * p.b_pitch + p.N - job.n0;
+  } else {
+    // The row tiles are gone through in bands of 1024 columns: the blocks
+    // that an XCD runs at a time then share rows and weights alike.
+    constexpr int kBand = 1024 / BN;
+    const int band = tile / (mt * kBand);
+    const int wide = min(kBand, nt - band * kBand);
+    tile -= band * mt * kBand;
+    job.n0 = (band * kBand + tile % wide) * BN;
+    tile /= wide;
+    const Segment seg = find_segment(p.offsets, p.G, p.M, tile, log2_of(BM));
+    if (seg.first >= seg.end) return false;
+    job.parted = false;
+    job.group = seg.group;
+    job.rows = min(BM, seg.end - seg.first);
+    job.steps = seg.group < p.G ? p.C : 0;
+    job.out_row = seg.first;
+    job.a = A + seg.first * p.a_pitch;
+    job.a_room = 0;
+    const long weights = (long)p.N * p.C;
+    job.b = B + min(seg.group, p.G - 1) * weights +
+            (MODE == kForward ? job.n0 * (long)p.C : job.n0);
+    job.b_room = (long)(p.C - 1) * p.N + p.N - job.n0;
+    if (seg.group < p.G - 1) job.b_room += weights;
+  }
+  job.cols = min(BN, p.N - job.n0);
+  return true;
+}
+
+// STAGES tiles of c in LDS (0: two, filled through registers).
 template <typename T, int BM, int BN, int WM, int WN, int MODE, int STAGES>
 __global__ __launch_bounds__(WM* WN * 64) void product_kernel(Product p) {
   constexpr int kThreads = WM * WN * 64;
-  constexpr int FM = BM / WM / 16, FN = BN / WN / 16;
-  typedef Tile<T, BM, MODE == kDWeight, kThreads, 1> TA;
-  typedef Tile<T, BN, MODE != kForward, kThreads, FN> TB;
+  constexpr int FM = BM / WM / 16, FN = BN / WN / 16, KS = 64;
+  typedef Tile<T, BM, KS, MODE == kDWeight, kThreads, 1> TA;
+  typedef Tile<T, BN, KS, MODE != kForward, kThreads, FN> TB;
   constexpr bool ASYNC = STAGES > 0;
   constexpr int kBuffers = ASYNC ? STAGES : 2;
   __shared__ __align__(16) char lds[kBuffers][TA::kBytes + TB::kBytes];
 
-  // Blocks go round the 8 XCDs: each gets a contiguous run of tiles, whose
+  // Blocks go round the 8 XCDs: each XCD gets a contiguous run of tiles, whose
   // operands its L2 then holds.
-  const int each = gridDim.x >> 3;
-  int tile = blockIdx.x;
-  if (tile < each * 8) tile = (tile & 7) * each + (tile >> 3);
-  const int nt = p.out ? (p.N + BN - 1) / BN : 1;
-  const int n0 = (tile % nt) * BN;
-  tile /= nt;
+  const int run = (p.tiles + 7) >> 3;
+  const int tile = (blockIdx.x & 7) * run + (blockIdx.x >> 3);
+  Job<T> job;
+  if (tile >= p.tiles || !find_job<T, BM, BN, MODE>(p, tile, job)) return;
 
-  const T* A = reinterpret_cast<const T*>(p.a);
-  const T* B = reinterpret_cast<const T*>(p.b);
-  int group, rows, steps;  // of out; steps of c
-  long out_row, a_room, b_room;
-  bool parted = false;
-  if (MODE == kDWeight) {
-    const int mt = (p.M + BM - 1) / BM;
-    const int unit = tile / mt;
-    const int m0 = (tile % mt) * BM;
-    int first, seg_start = 0;
-    if (p.shift) {
-      const Segment seg =
-          find_segment(p.offsets, p.G, p.C, unit, p.shift);
-      if (seg.first >= seg.end || seg.group >= p.G) return;
-      group = seg.group;
-      first = seg.first;
-      seg_start = seg.start;
-      steps = min(seg.end - first, 1 << p.shift);
-      parted = seg.end - seg.start > (1 << p.shift);
-    } else {
-      group = unit;
-      first = edge(p.offsets, group, p.G, p.C);
-      steps = edge(p.offsets, group + 1, p.G, p.C) - first;
-    }
-    rows = min(BM, p.M - m0);
-    out_row = (parted ? part_place(seg_start, p.shift) +
-                            ((first - seg_start) >> p.shift)
-                      : (long)group) *
-                  p.M +
-              m0;
-    A += first * p.a_pitch + m0;
-    B += first * p.b_pitch + n0;
-    a_room = (long)(p.C - first - 1) * p.a_pitch + p.M - m0;
-    b_room = (long)(p.C - first - 1) * p.b_pitch + p.N - n0;
-  } else {
-    const Segment seg =
-        find_segment(p.offsets, p.G, p.M, tile, log2_of(BM));
-    if (seg.first >= seg.end) return;
-    group = seg.group;
-    rows = min(BM, seg.end - seg.first);
-    steps = group < p.G ? p.C : 0;
-    out_row = seg.first;
-    A += seg.first * p.a_pitch;
-    a_room = 0;
-    const long weights = (long)p.N * p.C;
-    B += min(group, p.G - 1) * weights +
-         (MODE == kForward ? n0 * (long)p.C : n0);
-    b_room = (long)(p.C - 1) * p.N + p.N - n0;
-    if (group < p.G - 1) b_room += weights;
-  }
-  const int cols = min(BN, p.N - n0);
-  const long a_step = MODE == kDWeight ? kStep * p.a_pitch : kStep;
-  const long b_step = MODE == kForward ? kStep : kStep * p.b_pitch;
-
+  const long a_step = MODE == kDWeight ? KS * p.a_pitch : KS;
+  const long b_step = MODE == kForward ? KS : KS * p.b_pitch;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63;
   const int wm = (wave / WN) * (BM / WM), wn = (wave % WN) * (BN / WN);
-  f32x4 acc[FM][FN] = {};
-  f32x4 sum[FM] = {};
-  const bool sums = MODE == kDWeight && p.sums && n0 == 0 && wave % WN == 0;
-  typename Mma<T>::Frag ones;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) ones[i] = (T)1.f;
 
-  Vec<T> ra[ASYNC ? 1 : TA::kPer], rb[ASYNC ? 1 : TB::kPer];
-  // The tile's place at step c, and which of its granules are whole.
-  auto source = [&](int c, const T*& a, const T*& b,
-                    typename TA::Bounds& ba, typename TB::Bounds& bb) {
-    const long at = c / kStep;
-    a = A + at * a_step;
-    b = B + at * b_step;
-    ba = TA::bounds(p.a_pitch, rows, steps - c, a_room - at * a_step);
-    bb = TB::bounds(p.b_pitch, cols, steps - c, b_room - at * b_step);
-  };
-  auto load = [&](int c, int buf) {
+  // A tile's operands at step c, and which of their granules are whole.
+  struct Source {
     const T *a, *b;
     typename TA::Bounds ba;
     typename TB::Bounds bb;
-    source(c, a, b, ba, bb);
-    if constexpr (ASYNC) {
-      TA::load_async(a, p.a_pitch, ba, lds[buf]);
-      TB::load_async(b, p.b_pitch, bb, lds[buf] + TA::kBytes);
-    } else {
-      TA::load_regs(a, p.a_pitch, rows, steps - c, ba, ra);
-      TB::load_regs(b, p.b_pitch, cols, steps - c, bb, rb);
-    }
+    int steps;
   };
-  // Ends the loads of the tile at c: all but those of the `later` tiles that
-  // were issued behind them.
+  auto source = [&](int c) {
+    const long at = c / KS;
+    return Source{
+        job.a + at * a_step, job.b + at * b_step,
+        TA::bounds(p.a_pitch, job.rows, job.steps - c,
+                   job.a_room - at * a_step),
+        TB::bounds(p.b_pitch, job.cols, job.steps - c,
+                   job.b_room - at * b_step),
+        job.steps - c};
+  };
   constexpr int kLoads = TA::kPer + TB::kPer;
-  auto land = [&](int c, int buf, int later) {
+  constexpr int kAhead = ASYNC ? STAGES - 1 : 1;
+  Vec<T> ra[ASYNC ? 1 : TA::kPer], rb[ASYNC ? 1 : TB::kPer];
+  auto load = [&](const Source& s, int buf, int i) {
+    if (i < TA::kPer)
+      TA::load_async(s.a, p.a_pitch, s.ba, lds[buf], i);
+    else
+      TB::load_async(s.b, p.b_pitch, s.bb, lds[buf] + TA::kBytes,
+                     i - TA::kPer);
+  };
+  auto load_regs = [&](const auto& s) {
+    TA::load_regs(s.a, p.a_pitch, job.rows, s.steps, s.ba, ra);
+    TB::load_regs(s.b, p.b_pitch, job.cols, s.steps, s.bb, rb);
+  };
+  auto add = [](float& to, typename Mma<T>::Frag v) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) to += to_f(v[i]);
+  };
+
+  f32x4 acc[FM][FN] = {};
+  float sum[FM] = {};  // of this lane's steps; its neighbours have the rest
+  const bool sums =
+      MODE == kDWeight && p.sums && job.n0 == 0 && wave % WN == 0;
+  if (job.steps > 0) {
     if constexpr (ASYNC) {
-      wait_loads<kLoads, STAGES - 2>(later);
-      const T *a, *b;
-      typename TA::Bounds ba;
-      typename TB::Bounds bb;
-      source(c, a, b, ba, bb);
-      if (ba.ragged) TA::fill(a, p.a_pitch, rows, steps - c, ba, lds[buf]);
-      if (bb.ragged)
-        TB::fill(b, p.b_pitch, cols, steps - c, bb, lds[buf] + TA::kBytes);
+#pragma unroll
+      for (int s = 0; s < kAhead; ++s) {
+        const Source from = source(s * KS);
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) load(from, s, i);
+      }
+    } else {
+      load_regs(source(0));
+    }
+  }
+  int buf = 0;
+#pragma unroll 1
+  for (int c = 0; c < job.steps; c += KS) {
+    // Tile c lands.  At the barrier all waves have also read the tile
+    // before, whose place the loads of the tile kAhead further then take.
+    if constexpr (ASYNC) {
+      wait_loads<kLoads*(kAhead - 1)>();
+      const Source s = source(c);
+      if (s.ba.ragged)
+        TA::fill(s.a, p.a_pitch, job.rows, s.steps, s.ba, lds[buf]);
+      if (s.bb.ragged)
+        TB::fill(s.b, p.b_pitch, job.cols, s.steps, s.bb,
+                 lds[buf] + TA::kBytes);
     } else {
       TA::store_regs(ra, lds[buf]);
       TB::store_regs(rb, lds[buf] + TA::kBytes);
     }
     block_barrier();
-  };
-
-  constexpr int kAhead = ASYNC ? STAGES - 1 : 1;
-#pragma unroll
-  for (int s = 0; s < kAhead; ++s)
-    if (s * kStep < steps) load(s * kStep, s);
-  int buf = 0;
-  for (int c = 0; c < steps; c += kStep) {
-    const int later =
-        min(kAhead - 1, (steps - c - 1) / kStep);  // tiles behind this one
-    land(c, buf, later);
-    const int far = c + kAhead * kStep;
-    if (far < steps) load(far, (buf + kAhead) % kBuffers);
+    // Behind the last tile of all these loads write zeros, for nobody.
+    const Source next = source(c + kAhead * KS);
+    const int to = buf + kAhead >= kBuffers ? buf + kAhead - kBuffers
+                                            : buf + kAhead;
+    if constexpr (!ASYNC)
+      if (next.steps > 0) load_regs(next);
     const char* la = lds[buf];
     const char* lb = lds[buf] + TA::kBytes;
+    // 2 FM groups of FN matrix instructions.  Each group reads the fragments
+    // of the next and, in the first half, issues its share of the loads: all
+    // at once they would hold up the waves, since the vector memory takes
+    // them no faster than 64 bytes a clock.
+    typename Mma<T>::Frag fa[2], fb[2][FN];
 #pragma unroll
-    for (int h = 0; h < kStep; h += 32) {
-      typename Mma<T>::Frag fb[FN];
+    for (int j = 0; j < FN; ++j) fb[0][j] = TB::frag(lb, wn, j, 0);
+    fa[0] = TA::frag(la, wm, 0, 0);
 #pragma unroll
-      for (int j = 0; j < FN; ++j) fb[j] = TB::frag(lb, wn, j, h);
+    for (int g = 0; g < 2 * FM; ++g) {
+      const int h = g / FM, i = g % FM;
+      if (g + 1 < 2 * FM)
+        fa[(g + 1) & 1] = TA::frag(la, wm, (g + 1) % FM, (g + 1) / FM * 32);
+      if (h == 0) {
 #pragma unroll
-      for (int i = 0; i < FM; ++i) {
-        const typename Mma<T>::Frag fa = TA::frag(la, wm, i, h);
+        for (int j = i * FN / FM; j < (i + 1) * FN / FM; ++j)
+          fb[1][j] = TB::frag(lb, wn, j, 32);
+        if constexpr (ASYNC) {
 #pragma unroll
-        for (int j = 0; j < FN; ++j)
-          acc[i][j] = Mma<T>::go(fb[j], fa, acc[i][j]);
-        if (MODE == kDWeight && sums) sum[i] = Mma<T>::go(ones, fa, sum[i]);
+          for (int l = i * kLoads / FM; l < (i + 1) * kLoads / FM; ++l)
+            load(next, to, l);
+        }
       }
+#pragma unroll
+      for (int j = 0; j < FN; ++j)
+        acc[i][j] = Mma<T>::go(fb[h][j], fa[g & 1], acc[i][j]);
+      if (MODE == kDWeight && sums) add(sum[i], fa[g & 1]);
+      __builtin_amdgcn_sched_barrier(0);
     }
     buf = buf + 1 == kBuffers ? 0 : buf + 1;
   }
+
+  // LDS is not given back with loads under way.
+  if constexpr (ASYNC) wait_loads<0>();
 
   // lane: row m = lane & 15 of each fragment, 4 * FN neighbouring columns
   T* out = reinterpret_cast<T*>(p.out);
   const T* bias = reinterpret_cast<const T*>(p.bias);
   const int n = wn + (lane >> 4) * 4 * FN;
-  const int left = cols - n;
+  const int left = job.cols - n;
   if (left > 0 && (MODE != kDWeight || out)) {
-    float add[FN][4] = {};
-    if (MODE == kForward && bias && group < p.G) {
+    Vec<T> extra[FN / 2] = {};
+    const bool biased = MODE == kForward && bias && job.group < p.G;
+    if (biased) {
 #pragma unroll
-      for (int j = 0; j < FN * 4; ++j)
-        if (j < left)
-          add[j >> 2][j & 3] = to_f(bias[(long)group * p.N + n0 + n + j]);
+      for (int j = 0; j < FN / 2; ++j)
+        extra[j] = load_vec(bias + (long)job.group * p.N + job.n0 + n + j * 8,
+                            left - j * 8);
     }
 #pragma unroll
     for (int i = 0; i < FM; ++i) {
       const int m = wm + i * 16 + (lane & 15);
-      if (m >= rows) continue;
-      const long at = (out_row + m) * p.N + n0 + n;
-      if (MODE == kDWeight && parted) {
+      if (m >= job.rows) continue;
+      const long at = (job.out_row + m) * p.N + job.n0 + n;
+      if (MODE == kDWeight && job.parted) {
 #pragma unroll
         for (int j = 0; j < FN; ++j) {
           if (left >= j * 4 + 4) {
@@ -1418,24 +1472,29 @@ __global__ __launch_bounds__(WM* WN * 64) void product_kernel(Product p) {
         continue;
       }
 #pragma unroll
-      for (int j = 0; j < FN; j += 2) {
+      for (int j = 0; j < FN / 2; ++j) {
         Vec<T> v;
 #pragma unroll
-        for (int r = 0; r < 8; ++r)
-          v.v[r] = (T)(acc[i][j + r / 4][r & 3] + add[j + r / 4][r & 3]);
-        store_vec(out + at + j * 4, v, left - j * 4);
+        for (int r = 0; r < 8; ++r) {
+          float x = acc[i][j * 2 + r / 4][r & 3];
+          if (biased) x += to_f(extra[j].v[r]);
+          v.v[r] = (T)x;
+        }
+        store_vec(out + at + j * 8, v, left - j * 8);
       }
     }
   }
-  if (sums && lane < 16) {
+  if (sums) {
 #pragma unroll
     for (int i = 0; i < FM; ++i) {
+      sum[i] += __shfl_xor(sum[i], 16);
+      sum[i] += __shfl_xor(sum[i], 32);
       const int m = wm + i * 16 + lane;
-      if (m >= rows) continue;
-      if (parted)
-        p.part_sums[out_row + m] = sum[i][0];
+      if (lane >= 16 || m >= job.rows) continue;
+      if (job.parted)
+        p.part_sums[job.out_row + m] = sum[i];
       else
-        reinterpret_cast<T*>(p.sums)[out_row + m] = (T)sum[i][0];
+        reinterpret_cast<T*>(p.sums)[job.out_row + m] = (T)sum[i];
     }
   }
 }
@@ -1801,8 +1860,10 @@ void product_launch(Product p, at::TensorOptions opt) {
         mt = ((p.C >> p.shift) + p.G + 1) * m_tiles;
       }
     }
-    const long nt = p.out ? (p.N + bn - 1) / bn : 1;
-    kern<<<grid_of(mt * nt, threads), threads, 0, stream_now()>>>(p);
+    mt *= p.out ? (p.N + bn - 1) / bn : 1;
+    TORCH_CHECK(mt * threads < (1ll << 31), "too many tiles");
+    p.tiles = (int)mt;
+    kern<<<(unsigned)((mt + 7) / 8 * 8), threads, 0, stream_now()>>>(p);
     check_launch();
     if (MODE == kDWeight && p.shift) finish_launch<T>(p);
   };
@@ -1917,7 +1978,7 @@ at::Tensor product(const at::Tensor& a_in, const at::Tensor& weight,
         Product p{a.data_ptr(), weight.data_ptr(),
                   bias ? bias->data_ptr() : nullptr, out.data_ptr(), nullptr,
                   offsets.data_ptr<int>(), a.stride(0),
-                  transposed ? N : C, G, M, N, C, 0, nullptr, nullptr};
+                  transposed ? N : C, G, M, N, C, 0, nullptr, nullptr, 0};
         if (transposed)
           product_launch<T, kDRows>(p, a.options());
         else
@@ -1996,7 +2057,7 @@ grouped_linear_dweight(const at::Tensor& dy_in, const at::Tensor& rows_in,
   Product p{dy.data_ptr(), b.data_ptr(), nullptr,
             F && dw ? dw->data_ptr() : nullptr, db ? db->data_ptr() : nullptr,
             offsets.data_ptr<int>(), dy.stride(0), b.stride(0), G, N,
-            F ? F : N, M, 0, nullptr, nullptr};
+            F ? F : N, M, 0, nullptr, nullptr, 0};
   SKA_TYPES(dy.scalar_type(), [&] {
     if constexpr (sizeof(T) == 2) {
       product_launch<T, kDWeight>(p, dy.options());
