@@ -1356,15 +1356,17 @@ __global__ __launch_bounds__(WM* WN * 64) void product_kernel(Product p) {
     TA::load_regs(s.a, p.a_pitch, job.rows, s.steps, s.ba, ra);
     TB::load_regs(s.b, p.b_pitch, job.cols, s.steps, s.bb, rb);
   };
-  auto add = [](float& to, typename Mma<T>::Frag v) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) to += to_f(v[i]);
-  };
-
   f32x4 acc[FM][FN] = {};
-  float sum[FM] = {};  // of this lane's steps; its neighbours have the rest
-  const bool sums =
-      MODE == kDWeight && p.sums && job.n0 == 0 && wave % WN == 0;
+  // The sums over c of A: a product with ones, of which each of the WN waves
+  // that hold the same rows takes FS fragments.
+  constexpr int FS = FM / WN > 0 ? FM / WN : 1;
+  f32x4 sum[FS] = {};
+  const bool sums = MODE == kDWeight && p.sums && job.n0 == 0;
+  const int mine = wave % WN;
+  typename Mma<T>::Frag ones;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) ones[i] = (T)1.f;
+
   if (job.steps > 0) {
     if constexpr (ASYNC) {
 #pragma unroll
@@ -1429,7 +1431,8 @@ __global__ __launch_bounds__(WM* WN * 64) void product_kernel(Product p) {
 #pragma unroll
       for (int j = 0; j < FN; ++j)
         acc[i][j] = Mma<T>::go(fb[h][j], fa[g & 1], acc[i][j]);
-      if (MODE == kDWeight && sums) add(sum[i], fa[g & 1]);
+      if (MODE == kDWeight && sums && i / FS == mine)
+        sum[i % FS] = Mma<T>::go(ones, fa[g & 1], sum[i % FS]);
       __builtin_amdgcn_sched_barrier(0);
     }
     buf = buf + 1 == kBuffers ? 0 : buf + 1;
@@ -1484,17 +1487,15 @@ __global__ __launch_bounds__(WM* WN * 64) void product_kernel(Product p) {
       }
     }
   }
-  if (sums) {
+  if (sums && lane < 16) {
 #pragma unroll
-    for (int i = 0; i < FM; ++i) {
-      sum[i] += __shfl_xor(sum[i], 16);
-      sum[i] += __shfl_xor(sum[i], 32);
-      const int m = wm + i * 16 + lane;
-      if (lane >= 16 || m >= job.rows) continue;
+    for (int i = 0; i < FS; ++i) {
+      const int m = wm + (mine * FS + i) * 16 + lane;
+      if (mine * FS + i >= FM || m >= job.rows) continue;
       if (job.parted)
-        p.part_sums[job.out_row + m] = sum[i];
+        p.part_sums[job.out_row + m] = sum[i][0];
       else
-        reinterpret_cast<T*>(p.sums)[job.out_row + m] = (T)sum[i];
+        reinterpret_cast<T*>(p.sums)[job.out_row + m] = (T)sum[i][0];
     }
   }
 }
