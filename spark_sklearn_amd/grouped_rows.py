@@ -34,8 +34,10 @@ __all__ = ["GroupPlan", "group_rows", "gather_rows", "combine_rows",
            "grouped_linear"]
 
 _MAX_GROUPS = (1 << 24) - 1
+_NO_PLAN = "plan must be a GroupPlan (see group_rows)"
 _MAX_WIDTH = (1 << 21) - 1
 _reference: Any = None
+_ext: Any = None
 
 
 class GroupPlan(NamedTuple):
@@ -69,11 +71,9 @@ def _check_rows(name, t):
     import torch
 
     _require(_is_tensor(t), TypeError, f"{name} must be a torch.Tensor")
-    allowed = (torch.float32, torch.bfloat16, torch.float16)
-    if not t.is_cuda:
-        allowed += (torch.float64,)
-        _require(t.device.type == "cpu", ValueError,
-                 f"{name} must be on a GPU or the CPU, got {t.device}")
+    allowed = (torch.float64, torch.float32, torch.bfloat16, torch.float16)
+    _require(t.device.type == "cpu", ValueError,
+             f"{name} must be on a GPU or the CPU, got {t.device}")
     _require(t.dtype in allowed, TypeError,
              f"{name} must be one of {allowed}, got {t.dtype}")
     _require(t.dim() == 2, ValueError,
@@ -97,8 +97,6 @@ def _check_ints(name, t, device, dim=None):
 
 
 def _check_plan(plan, device):
-    _require(isinstance(plan, GroupPlan), TypeError,
-             "plan must be a GroupPlan (see group_rows)")
     _check_ints("plan.offsets", plan.offsets, device, 1)
     _check_ints("plan.slots", plan.slots, device)
     _require(plan.offsets.numel() >= 2, ValueError,
@@ -111,17 +109,26 @@ def _check_plan(plan, device):
     return plan.offsets.contiguous(), slots.contiguous()
 
 
+def _native(t):
+    """The kernels, where the tensor is on a GPU.  They make the checks that
+    are made here for the reference, with the same exceptions."""
+    global _ext
+    if getattr(t, "is_cuda", False):
+        if _ext is None:
+            from .ops import load_extension
+
+            _ext = load_extension()
+        return _ext
+    return None
+
+
 def _kernels(t):
     """The functions that serve the tensor, each with its gradients: native
     kernels on a GPU, the reference on the CPU."""
-    if t.is_cuda:
-        from .ops import load_extension
-
-        return load_extension()
     global _reference
     if _reference is None:
         _reference = _make_reference()
-    return _reference
+    return _native(t) or _reference
 
 
 def _make_reference():
@@ -197,6 +204,10 @@ def group_rows(ids, n_groups: int) -> GroupPlan:
     n_groups : int
         Up to 2^24 - 1.
     """
+    if type(n_groups) is int:
+        native = _native(ids)
+        if native is not None and n_groups.bit_length() < 64:
+            return GroupPlan(*native.group_rows(ids, n_groups))
     import torch
 
     _require(_is_tensor(ids), TypeError, "ids must be a torch.Tensor")
@@ -222,6 +233,10 @@ def gather_rows(x, plan: GroupPlan):
     ``plan.offsets[-1]`` (entries without a group) are zero.  Differentiable
     in ``x``.
     """
+    native = _native(x)
+    if native is not None and isinstance(plan, GroupPlan):
+        return native.gather_rows(x, plan.offsets, plan.slots)
+    _require(isinstance(plan, GroupPlan), TypeError, _NO_PLAN)
     _check_rows("x", x)
     offsets, slots = _check_plan(plan, x.device)
     _require(slots.shape[0] == x.shape[0], ValueError,
@@ -239,8 +254,12 @@ def combine_rows(rows, plan: GroupPlan, weights=None):
     zero.  Sums run over j in order, in 32 bits.  Differentiable in ``rows``
     and ``weights``.
     """
+    native = _native(rows)
+    if native is not None and isinstance(plan, GroupPlan):
+        return native.combine_rows(rows, plan.offsets, plan.slots, weights)
     import torch
 
+    _require(isinstance(plan, GroupPlan), TypeError, _NO_PLAN)
     _check_rows("rows", rows)
     offsets, slots = _check_plan(plan, rows.device)
     _require(slots.numel() == rows.shape[0], ValueError,
@@ -280,6 +299,9 @@ def grouped_linear(rows, weight, offsets, bias: Optional[Any] = None):
     in ``rows``, ``weight`` and ``bias``; an empty group's gradients are
     zero.
     """
+    native = _native(rows)
+    if native is not None:
+        return native.grouped_linear(rows, weight, offsets, bias)
     _check_rows("rows", rows)
     _require(_is_tensor(weight) and (bias is None or _is_tensor(bias)),
              TypeError, "weight and bias must be torch.Tensors")
