@@ -886,134 +886,9 @@ __host__ __device__ constexpr int log2_of(int v) {
   return v <= 1 ? 0 : 1 + log2_of(v >> 1);
 }
 
-// The plain tile: 64 x 64 outputs, 32 steps of the contraction at a time in
-// 32 bits through LDS, v_mfma_f32_16x16x4_f32.  Operands have any strides.
-constexpr int kTile = 64, kDepth = 32, kPitch = 36;
-
-template <typename T>
-__device__ __forceinline__ void load_tile(const T* src, long s_row, long s_k,
-                                          int rows, int depth,
-                                          float (*dst)[kPitch]) {
-  const int tid = threadIdx.x;
-  for (int e = tid; e < kTile * kDepth; e += 256) {
-    const int r = s_k == 1 ? e / kDepth : e % kTile;
-    const int c = s_k == 1 ? e % kDepth : e / kTile;
-    dst[r][c] =
-        r < rows && c < depth ? to_f(src[r * s_row + c * s_k]) : 0.f;
-  }
-}
-
-__device__ __forceinline__ void tile_products(const float (*a)[kPitch],
-                                              const float (*b)[kPitch],
-                                              f32x4 (&acc)[2][2]) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int r = lane & 15, q = lane >> 4;
-  const int m0 = (wave >> 1) * 32, n0 = (wave & 1) * 32;
-#pragma unroll
-  for (int c = 0; c < kDepth; c += 16) {
-    f32x4 av[2], bv[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      av[i] = *reinterpret_cast<const f32x4*>(&a[m0 + i * 16 + r][c + q * 4]);
-      bv[i] = *reinterpret_cast<const f32x4*>(&b[n0 + i * 16 + r][c + q * 4]);
-    }
-#pragma unroll
-    for (int s = 0; s < 4; ++s)
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-          acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(
-              av[i][s], bv[j][s], acc[i][j], 0, 0, 0);
-  }
-}
-
-// out[s, n] = sum_c a[s, c] * w[g(s)][n * s_n + c * s_c] (+ bias[g(s), n])
-template <typename T>
-__global__ __launch_bounds__(256) void product_plain_kernel(
-    const T* __restrict__ a, long a_pitch, const T* __restrict__ w,
-    long w_group, long s_n, long s_c, const T* __restrict__ bias,
-    const int* __restrict__ offsets, int G, int M, int N, int C,
-    T* __restrict__ out) {
-  const Segment seg =
-      find_segment(offsets, G, M, blockIdx.x, log2_of(kTile));
-  if (seg.first >= seg.end) return;
-  __shared__ __align__(16) float As[kTile][kPitch], Bs[kTile][kPitch];
-  const int rows = min(kTile, seg.end - seg.first);
-  const int n0 = blockIdx.y * kTile;
-  const int cols = min(kTile, N - n0);
-  f32x4 acc[2][2] = {};
-  if (seg.group < G) {
-    const T* ga = a + seg.first * a_pitch;
-    const T* gw = w + seg.group * w_group + n0 * s_n;
-    for (int c = 0; c < C; c += kDepth) {
-      __syncthreads();
-      load_tile(ga + c, a_pitch, 1, rows, C - c, As);
-      load_tile(gw + c * s_c, s_n, s_c, cols, C - c, Bs);
-      __syncthreads();
-      tile_products(As, Bs, acc);
-    }
-  }
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-  for (int i = 0; i < 2; ++i)
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int m = (wave >> 1) * 32 + i * 16 + (lane >> 4) * 4 + r;
-        const int n = (wave & 1) * 32 + j * 16 + (lane & 15);
-        if (m >= rows || n >= cols) continue;
-        float v = acc[i][j][r];
-        if (bias && seg.group < G)
-          v += to_f(bias[(long)seg.group * N + n0 + n]);
-        out[(long)(seg.first + m) * N + n0 + n] = (T)v;
-      }
-}
-
-// dw[g, n, f] = sum over the group's rows of dy[s, n] * x[s, f]; the blocks
-// of the first column tile sum db[g, n] too.
-template <typename T>
-__global__ __launch_bounds__(256) void weights_plain_kernel(
-    const T* __restrict__ dy, long dy_pitch, const T* __restrict__ x,
-    long x_pitch, const int* __restrict__ offsets, int G, int M, int N, int F,
-    T* __restrict__ dw, T* __restrict__ db) {
-  __shared__ __align__(16) float As[kTile][kPitch], Bs[kTile][kPitch];
-  const int g = blockIdx.x;
-  const int n0 = blockIdx.y * kTile;
-  const int f0 = blockIdx.z * kTile;
-  const int first = edge(offsets, g, G, M), end = edge(offsets, g + 1, G, M);
-  const int ns = min(kTile, N - n0), fs = min(kTile, F - f0);
-  f32x4 acc[2][2] = {};
-  float sum = 0.f;
-  for (int s = first; s < end; s += kDepth) {
-    __syncthreads();
-    load_tile(dy + (long)s * dy_pitch + n0, 1, dy_pitch, ns, end - s, As);
-    load_tile(x + (long)s * x_pitch + f0, 1, x_pitch, fs, end - s, Bs);
-    __syncthreads();
-    tile_products(As, Bs, acc);
-    if (threadIdx.x < kTile)
-      for (int c = 0; c < kDepth; ++c) sum += As[threadIdx.x][c];
-  }
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-  for (int i = 0; i < 2; ++i)
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int n = (wave >> 1) * 32 + i * 16 + (lane >> 4) * 4 + r;
-        const int f = (wave & 1) * 32 + j * 16 + (lane & 15);
-        if (n < ns && f < fs)
-          dw[((long)g * N + n0 + n) * F + f0 + f] = (T)acc[i][j][r];
-      }
-  if (db && blockIdx.z == 0 && threadIdx.x < ns)
-    db[(long)g * N + n0 + threadIdx.x] = (T)sum;
-}
-
-
 // ---------------------------------------------------------------------------
-// 16-bit products on v_mfma_f32_16x16x32.  All three are
+// Products on v_mfma_f32_16x16x32 (16-bit types) and v_mfma_f32_16x16x4
+// (float32).  All three are
 //
 //     out[m, n] = sum_c A[m, c] * B[n, c]
 //
@@ -1022,13 +897,17 @@ __global__ __launch_bounds__(256) void weights_plain_kernel(
 //   dweight   A = dy   (m = n', c = s)   B = rows      (n = f, c = s)
 //
 // An operand lies in memory along c ("along") or across it ("across": m or n
-// is the contiguous index).  Tiles of 64 steps of c go to LDS in granules of
-// 8 values, by buffer loads that write LDS themselves; a lane out of range
-// writes zeros.  An along tile is [m][64]: granule j of row m lies at
-// j ^ (m & 7), and a fragment is one 16-byte read.  An across tile is
-// [64][m]: its fragments are two transposing reads of 4 values of c each
-// (16 lanes read 4 rows of 32 bytes), and granules are moved by bits of c so
-// that these rows lie in different banks.
+// is the contiguous index).  Tiles of 128 bytes of c (KS steps) go to LDS in
+// granules of 16 bytes (V values), by buffer loads that write LDS themselves; a
+// lane out of range writes zeros.  An along tile is [m][KS]: granule j of row m
+// lies at j ^ swap(m), and a fragment is one 16-byte read.  An across tile is
+// [KS][m]: its fragments are two transposing reads of 4 values of c each (16
+// lanes read 4 rows of 32 bytes), or 4 single reads of float32; granules are
+// moved by bits of c so that these rows lie in different banks.
+//
+// A lane of either operand holds the V steps from (lane >> 4) * V of a half
+// tile.  That both agree is all that the sum needs: for float32, four
+// instructions take one of the four steps each.
 //
 // The matrix instruction gets B first: a lane then holds 4 neighbouring n of
 // one m, and stores them together.
@@ -1052,6 +931,17 @@ struct Mma<_Float16> {
   }
 };
 
+template <>
+struct Mma<float> {
+  typedef f32x4 Frag;
+  static __device__ __forceinline__ f32x4 go(Frag a, Frag b, f32x4 c) {
+#pragma unroll
+    for (int s = 0; s < 4; ++s)
+      c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[s], b[s], c, 0, 0, 0);
+    return c;
+  }
+};
+
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
@@ -1061,22 +951,29 @@ typedef int i32x4 __attribute__((ext_vector_type(4)));
 // the rows of FRAGS neighbouring fragments are dealt out 4 at a time: row r of
 // fragment j is (r / 4) * 4 * FRAGS + j * 4 + r % 4 of their 16 * FRAGS.  A
 // lane of the product then holds 4 * FRAGS neighbouring n.
-template <typename T, int EXT, int KS, bool ACROSS, int THREADS, int FRAGS>
+template <typename T, int EXT, bool ACROSS, int THREADS, int FRAGS>
 struct Tile {
-  static constexpr int kGranules = EXT * KS / 8;
+  static constexpr int V = 16 / sizeof(T);
+  static constexpr int KS = 8 * V;
+  static constexpr int kGranules = EXT * KS / V;
   static constexpr int kPer = kGranules / THREADS;
-  static constexpr int kAcross = EXT / 8;  // granules of one step of c
-  static constexpr int kBytes = EXT * KS * 2;
+  static constexpr int kAcross = EXT / V;  // granules of one step of c
+  static constexpr int kBytes = kGranules * 16;
 
   // how the granules of an along row, or of an across step, are moved, so
   // that the 8 rows of 8 lanes (the 4 steps of 16) lie in different banks
-  static constexpr int kAlong = KS / 8;  // granules of one along row
   static __device__ __forceinline__ int swap(int row) {
     const int high = FRAGS == 1 ? row >> 2 : FRAGS == 2 ? row >> 3 : row >> 4;
-    if (KS == 32) return ((row >> 1) & 1) | (high & 1) << 1;
     return (row & 3) | (high & 1) << 2;
   }
   static __device__ __forceinline__ int move(int c) {
+    if (V == 4) {
+      const int q = (c >> 2) & 3;
+      return (FRAGS == 1   ? q << 2
+              : FRAGS == 2 ? (q & 1) | (q & 2) << 2
+                           : q) &
+             (kAcross - 1);
+    }
     if (FRAGS == 1)
       return (((c & 3) << 1) | (((c >> 3) & 1) << 3)) & (kAcross - 1);
     if (FRAGS == 2)
@@ -1087,10 +984,10 @@ struct Tile {
   static __device__ __forceinline__ void place(int g, int& row, int& c) {
     if (ACROSS) {
       c = g / kAcross;
-      row = ((g % kAcross) ^ move(c)) * 8;
+      row = ((g % kAcross) ^ move(c)) * V;
     } else {
-      row = g / kAlong;
-      c = ((g % kAlong) ^ swap(row)) * 8;
+      row = g >> 3;
+      c = ((g & 7) ^ swap(row)) * V;
     }
   }
   static __device__ __forceinline__ long at(int row, int c, long pitch) {
@@ -1107,12 +1004,12 @@ struct Tile {
   static __device__ __forceinline__ Bounds bounds(long pitch, int rows,
                                                   int steps, long room) {
     if (ACROSS) {
-      const bool cut = (rows & 7) && (min(steps, KS) - 1) * pitch +
-                                             ((rows + 7) & ~7) >
-                                         room;
-      return {cut ? rows & ~7 : rows, steps, cut};
+      const bool cut = rows % V && (min(steps, KS) - 1) * pitch +
+                                           ((rows + V - 1) & -V) >
+                                       room;
+      return {cut ? rows & -V : rows, steps, cut};
     }
-    return {rows, steps & ~7, steps < KS && (steps & 7)};
+    return {rows, steps & -V, steps < KS && steps % V};
   }
   // One of a wave's kPer loads.  Written in assembly, because the compiler
   // would wait for all loads under way before it reads LDS; whoever reads the
@@ -1131,7 +1028,8 @@ struct Tile {
     int row, c;
     place(i * THREADS + wave * 64 + lane, row, c);
     const bool in = row < b.rows && c < b.steps;
-    const unsigned off = in ? (unsigned)at(row, c, pitch) * 2 : 0x80000000u;
+    const unsigned off = in ? (unsigned)at(row, c, pitch) * (unsigned)sizeof(T)
+                            : 0x80000000u;
     asm volatile(
         "s_mov_b32 m0, %0\n\t"
         "s_nop 0\n\t"
@@ -1152,7 +1050,7 @@ struct Tile {
                            : (c >= b.steps && row < rows ? steps - c : 0);
       T* to = reinterpret_cast<T*>(lds + g * 16);
       const T* from = src + at(row, c, pitch);
-      for (int e = 0; e < min(n, 8); ++e) to[e] = from[e];
+      for (int e = 0; e < min(n, V); ++e) to[e] = from[e];
     }
   }
   // rows that begin at odd addresses: through registers
@@ -1164,7 +1062,7 @@ struct Tile {
     for (int i = 0; i < kPer; ++i) {
       int row, c;
       place(i * THREADS + threadIdx.x, row, c);
-      int n = row < b.rows && c < b.steps ? 8 : 0;
+      int n = row < b.rows && c < b.steps ? V : 0;
       if (b.ragged && n == 0 && row < rows && c < steps)
         n = ACROSS ? rows - row : steps - c;
       v[i] = load_vec(src + (n > 0 ? at(row, c, pitch) : 0), n);
@@ -1177,19 +1075,20 @@ struct Tile {
       *reinterpret_cast<Vec<T>*>(lds + (i * THREADS + threadIdx.x) * 16) =
           v[i];
   }
-  // fragment j of the rows from row0 and the steps [c0, c0 + 32)
+  // fragment j of the rows from row0, in a half of the tile's steps
   static __device__ __forceinline__ typename Mma<T>::Frag frag(
-      const char* lds, int row0, int j, int c0) {
+      const char* lds, int row0, int j, int half) {
     const int lane = threadIdx.x & 63;
     const int r = lane & 15, q = lane >> 4;
-    if (ACROSS) {
+    const int c0 = half * (KS / 2) + q * V;
+    if constexpr (ACROSS && V == 8) {
       // lane (4 * step + s) of 16 reads rows 4 * s .. 4 * s + 3 of the fragment
       const int row = row0 + (FRAGS == 1 ? j * 16 + (r & 3) * 4
                                          : (r & 3) * 4 * FRAGS + j * 4);
       s16x4 v[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const int c = c0 + q * 8 + h * 4 + (r >> 2);
+        const int c = c0 + h * 4 + (r >> 2);
         const int g = (row >> 3) ^ move(c);
         v[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
             SKA_LDS(s16x4, lds + (c * kAcross + g) * 16 + (row & 4) * 2));
@@ -1201,8 +1100,18 @@ struct Tile {
     const int row = row0 + (FRAGS == 1 ? j * 16 + r
                                        : (r >> 2) * 4 * FRAGS + j * 4 +
                                              (r & 3));
+    if constexpr (ACROSS) {
+      typename Mma<T>::Frag v;
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const int g = (row / V) ^ move(c0 + i);
+        v[i] = *reinterpret_cast<const T*>(
+            lds + ((c0 + i) * kAcross + g) * 16 + row % V * sizeof(T));
+      }
+      return v;
+    }
     return *reinterpret_cast<const typename Mma<T>::Frag*>(
-        lds + (row * kAlong + (((c0 >> 3) + q) ^ swap(row))) * 16);
+        lds + (row * 8 + ((c0 / V) ^ swap(row))) * 16);
   }
 };
 
@@ -1321,9 +1230,10 @@ __device__ __forceinline__ bool find_job(const Product& p, int tile,
 template <typename T, int BM, int BN, int WM, int WN, int MODE, int STAGES>
 __global__ __launch_bounds__(WM* WN * 64) void product_kernel(Product p) {
   constexpr int kThreads = WM * WN * 64;
-  constexpr int FM = BM / WM / 16, FN = BN / WN / 16, KS = 64;
-  typedef Tile<T, BM, KS, MODE == kDWeight, kThreads, 1> TA;
-  typedef Tile<T, BN, KS, MODE != kForward, kThreads, FN> TB;
+  constexpr int FM = BM / WM / 16, FN = BN / WN / 16;
+  typedef Tile<T, BM, MODE == kDWeight, kThreads, 1> TA;
+  typedef Tile<T, BN, MODE != kForward, kThreads, FN> TB;
+  constexpr int KS = TA::KS;
   constexpr bool ASYNC = STAGES > 0;
   constexpr int kBuffers = ASYNC ? STAGES : 2;
   __shared__ __align__(16) char lds[kBuffers][TA::kBytes + TB::kBytes];
@@ -1381,7 +1291,7 @@ __global__ __launch_bounds__(WM* WN * 64) void product_kernel(Product p) {
   const int mine = wave % WN;
   typename Mma<T>::Frag ones;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) ones[i] = (T)1.f;
+  for (int i = 0; i < TA::V; ++i) ones[i] = (T)1.f;
 
   if (job.steps > 0) {
     if constexpr (ASYNC) {
@@ -1433,11 +1343,11 @@ __global__ __launch_bounds__(WM* WN * 64) void product_kernel(Product p) {
     for (int g = 0; g < 2 * FM; ++g) {
       const int h = g / FM, i = g % FM;
       if (g + 1 < 2 * FM)
-        fa[(g + 1) & 1] = TA::frag(la, wm, (g + 1) % FM, (g + 1) / FM * 32);
+        fa[(g + 1) & 1] = TA::frag(la, wm, (g + 1) % FM, (g + 1) / FM);
       if (h == 0) {
 #pragma unroll
         for (int j = i * FN / FM; j < (i + 1) * FN / FM; ++j)
-          fb[1][j] = TB::frag(lb, wn, j, 32);
+          fb[1][j] = TB::frag(lb, wn, j, 1);
         if constexpr (ASYNC) {
 #pragma unroll
           for (int l = i * kLoads / FM; l < (i + 1) * kLoads / FM; ++l)
@@ -1463,13 +1373,14 @@ __global__ __launch_bounds__(WM* WN * 64) void product_kernel(Product p) {
   const int n = wn + (lane >> 4) * 4 * FN;
   const int left = job.cols - n;
   if (left > 0 && (MODE != kDWeight || out)) {
-    Vec<T> extra[FN / 2] = {};
+    constexpr int V = TA::V, kStores = 4 * FN / V;
+    Vec<T> extra[kStores] = {};
     const bool biased = MODE == kForward && bias && job.group < p.G;
     if (biased) {
 #pragma unroll
-      for (int j = 0; j < FN / 2; ++j)
-        extra[j] = load_vec(bias + (long)job.group * p.N + job.n0 + n + j * 8,
-                            left - j * 8);
+      for (int j = 0; j < kStores; ++j)
+        extra[j] = load_vec(bias + (long)job.group * p.N + job.n0 + n + j * V,
+                            left - j * V);
     }
 #pragma unroll
     for (int i = 0; i < FM; ++i) {
@@ -1491,15 +1402,15 @@ __global__ __launch_bounds__(WM* WN * 64) void product_kernel(Product p) {
         continue;
       }
 #pragma unroll
-      for (int j = 0; j < FN / 2; ++j) {
+      for (int j = 0; j < kStores; ++j) {
         Vec<T> v;
 #pragma unroll
-        for (int r = 0; r < 8; ++r) {
-          float x = acc[i][j * 2 + r / 4][r & 3];
+        for (int r = 0; r < V; ++r) {
+          float x = acc[i][(j * V + r) / 4][r & 3];
           if (biased) x += to_f(extra[j].v[r]);
           v.v[r] = (T)x;
         }
-        store_vec(out + at + j * 8, v, left - j * 8);
+        store_vec(out + at + j * V, v, left - j * V);
       }
     }
   }
@@ -1554,17 +1465,7 @@ __global__ __launch_bounds__(256) void finish_kernel(Product p) {
 // ---------------------------------------------------------------------------
 template <typename T>
 struct Wide {
-  typedef typename Vec<T>::Values Frag;
-  static __device__ __forceinline__ f32x4 go(Frag a, Frag b, f32x4 c) {
-    if constexpr (sizeof(T) == 2) {
-      return Mma<T>::go(a, b, c);
-    } else {
-#pragma unroll
-      for (int s = 0; s < 4; ++s)
-        c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[s], b[s], c, 0, 0, 0);
-      return c;
-    }
-  }
+  typedef typename Mma<T>::Frag Frag;
   static __device__ __forceinline__ Frag load(const T* p) {
     return get(p).v;
   }
@@ -1623,7 +1524,7 @@ __global__ __launch_bounds__(256) void narrow_kernel(Product p, bool by_row) {
         for (int i = 0; i < MF; ++i)
 #pragma unroll
           for (int j = 0; j < NF; ++j)
-            acc[i][j] = Wide<T>::go(fb[u][j], fa[u][i], acc[i][j]);
+            acc[i][j] = Mma<T>::go(fb[u][j], fa[u][i], acc[i][j]);
     };
     constexpr int U = MF + NF > 4 ? 2 : 4;
     for (; c + (U - 1) * KW * kChunk < whole; c += U * KW * kChunk)
@@ -1640,7 +1541,7 @@ __global__ __launch_bounds__(256) void narrow_kernel(Product p, bool by_row) {
       for (int i = 0; i < MF; ++i)
 #pragma unroll
         for (int j = 0; j < NF; ++j)
-          acc[i][j] = Wide<T>::go(fb[j], fa[i], acc[i][j]);
+          acc[i][j] = Mma<T>::go(fb[j], fa[i], acc[i][j]);
     }
   }
   if constexpr (KW > 1) {
@@ -1900,6 +1801,13 @@ void product_launch(Product p, at::TensorOptions opt) {
     const bool large = p.G * tiles(256) >= 192 &&
                        tiles(256) * 65536 * 3 <= 4l * p.M * p.N;
     const bool middle = p.M > 64 && p.N > 64 && p.G * tiles(128) >= 256;
+    if constexpr (sizeof(T) == 4) {
+      if (middle)
+        go(product_kernel<T, 128, 128, 2, 2, MODE, 2>, 128, 128, 256);
+      else
+        go(product_kernel<T, 64, 64, 2, 2, MODE, 3>, 64, 64, 256);
+      return;
+    }
     if (async && large)
       go(product_kernel<T, 256, 256, 2, 4, MODE, 2>, 256, 256, 512);
     else if (async && middle)
@@ -1918,6 +1826,14 @@ void product_launch(Product p, at::TensorOptions opt) {
   };
   const bool large = each >= 768 && p.N > 128 && row_tiles(256, 256) >= 512;
   const bool middle = each >= 192 && p.N > 64 && row_tiles(128, 128) >= 256;
+  if constexpr (sizeof(T) == 4) {
+    // 128^2 tiles reach the matrix units' rate in float32
+    if (p.N > 64 && each >= 64 && row_tiles(128, 128) >= 256)
+      go(product_kernel<T, 128, 128, 2, 2, MODE, 2>, 128, 128, 256);
+    else
+      go(product_kernel<T, 64, 64, 2, 2, MODE, 3>, 64, 64, 256);
+    return;
+  }
   if (async && large)
     go(product_kernel<T, 256, 256, 2, 4, MODE, 2>, 256, 256, 512);
   else if (async && middle)
@@ -1964,37 +1880,15 @@ at::Tensor product(const at::Tensor& a_in, const at::Tensor& weight,
   const int M = (int)a.size(0);
   at::Tensor out = at::empty({M, N}, a.options());
   if (out.numel() == 0) return out;
-  if (a.scalar_type() != at::kFloat) {
-    SKA_TYPES(a.scalar_type(), [&] {
-      if constexpr (sizeof(T) == 2) {
-        Product p{a.data_ptr(), weight.data_ptr(),
-                  bias ? bias->data_ptr() : nullptr, out.data_ptr(), nullptr,
-                  offsets.data_ptr<int>(), a.stride(0),
-                  transposed ? N : C, G, M, N, C, 0, nullptr, nullptr, 0};
-        if (transposed)
-          product_launch<T, kDRows>(p, a.options());
-        else
-          product_launch<T, kForward>(p, a.options());
-      }
-    });
-    return out;
-  }
-  if (!transposed &&
-      narrow_launch<float>(
-          Product{a.data_ptr(), weight.data_ptr(),
-                  bias ? bias->data_ptr() : nullptr, out.data_ptr(), nullptr,
-                  offsets.data_ptr<int>(), a.stride(0), C, G, M, N, C, 0,
-                  nullptr, nullptr}))
-    return out;
+  Product p{a.data_ptr(), weight.data_ptr(),
+            bias ? bias->data_ptr() : nullptr, out.data_ptr(), nullptr,
+            offsets.data_ptr<int>(), a.stride(0), transposed ? N : C, G, M, N,
+            C, 0, nullptr, nullptr, 0};
   SKA_TYPES(a.scalar_type(), [&] {
-    dim3 grid(M / kTile + G + 1, (N + kTile - 1) / kTile);
-    TORCH_CHECK(grid.y < 65536, "rows are too wide");
-    product_plain_kernel<T><<<grid, 256, 0, stream_now()>>>(
-        ptr<T>(a), a.stride(0), ptr<T>(weight), (long)N * C,
-        transposed ? 1 : C, transposed ? N : 1,
-        bias ? ptr<T>(*bias) : nullptr, offsets.data_ptr<int>(), G, M, N, C,
-        ptr<T>(out));
-    check_launch();
+    if (transposed)
+      product_launch<T, kDRows>(p, a.options());
+    else
+      product_launch<T, kForward>(p, a.options());
   });
   return out;
 }
@@ -2038,19 +1932,10 @@ grouped_linear_dweight(const at::Tensor& dy_in, const at::Tensor& rows_in,
             offsets.data_ptr<int>(), dy.stride(0), b.stride(0), G, N,
             F ? F : N, M, 0, nullptr, nullptr, 0};
   SKA_TYPES(dy.scalar_type(), [&] {
-    if constexpr (sizeof(T) == 2) {
-      product_launch<T, kDWeight>(p, dy.options());
-    } else if (N <= 64 || !p.out) {
+    if (sizeof(T) == 4 && N <= 64)
       narrow_dweight_launch(p, dy.options());
-    } else {
-      dim3 grid(G, (N + kTile - 1) / kTile, (F + kTile - 1) / kTile);
-      TORCH_CHECK(grid.y < 65536 && grid.z < 65536, "rows are too wide");
-      weights_plain_kernel<T><<<grid, 256, 0, stream_now()>>>(
-          ptr<T>(dy), dy.stride(0), ptr<T>(x), x.stride(0),
-          offsets.data_ptr<int>(), G, M, N, F, ptr<T>(*dw),
-          db ? ptr<T>(*db) : nullptr);
-      check_launch();
-    }
+    else
+      product_launch<T, kDWeight>(p, dy.options());
   });
   return {dw, db};
 }
@@ -2109,11 +1994,13 @@ struct CombineFunction : torch::autograd::Function<CombineFunction> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     auto saved = ctx->get_saved_variables();
-    const bool need_weights = ctx->saved_data["weights"].toBool();
+    const bool need_weights =
+        ctx->saved_data["weights"].toBool() && ctx->needs_input_grad(3);
     auto got = combine_rows_backward(
         grads[0], need_weights ? saved[0] : grads[0], saved[1], saved[2],
         saved[3].defined() ? Maybe(saved[3]) : Maybe(),
-        ctx->saved_data["rows"].toBool(), need_weights);
+        ctx->saved_data["rows"].toBool() && ctx->needs_input_grad(0),
+        need_weights);
     return once({defined_or_none(std::get<0>(got)), at::Tensor(),
                  at::Tensor(), defined_or_none(std::get<1>(got)),
                  at::Tensor(), at::Tensor()});
@@ -2137,11 +2024,13 @@ struct LinearFunction : torch::autograd::Function<LinearFunction> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     auto saved = ctx->get_saved_variables();
     at::Tensor drows;
-    if (ctx->saved_data["rows"].toBool())
+    if (ctx->saved_data["rows"].toBool() && ctx->needs_input_grad(0))
       drows = grouped_linear_drows(grads[0], saved[1], saved[2]);
     std::tuple<Maybe, Maybe> got;
-    const bool need_weight = ctx->saved_data["weight"].toBool();
-    const bool need_bias = ctx->saved_data["bias"].toBool();
+    const bool need_weight =
+        ctx->saved_data["weight"].toBool() && ctx->needs_input_grad(1);
+    const bool need_bias =
+        ctx->saved_data["bias"].toBool() && ctx->needs_input_grad(3);
     if (need_weight || need_bias)
       got = grouped_linear_dweight(grads[0], saved[0], saved[2], need_weight,
                                    need_bias);

@@ -382,6 +382,21 @@ def test_grouped_linear_some_gradients(device, wrt):
         assert torch.equal(got, every[i])
 
 
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("wrt", [(0,), (1,), (2,), (3,), (1, 3)])
+def test_gradients_asked_for_one_by_one(device, wrt):
+    """Some gradients of a run in which all inputs require theirs."""
+    x, ids, weight, bias, w, dy = chain_data(device, T=50)
+    leaves = [v.requires_grad_() for v in (x, weight, bias, w)]
+    every = torch.autograd.grad(
+        chain(x, ids, weight.shape[0], weight, bias, w), leaves, dy)
+    some = torch.autograd.grad(
+        chain(x, ids, weight.shape[0], weight, bias, w),
+        [leaves[i] for i in wrt], dy)
+    for got, i in zip(some, wrt):
+        assert torch.equal(got, every[i])
+
+
 def test_gradcheck_reference():
     """The reference's gradients against differences, in 64 bits."""
     gen = torch.Generator().manual_seed(5)
