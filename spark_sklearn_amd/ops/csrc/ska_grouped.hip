@@ -1589,11 +1589,12 @@ __global__ __launch_bounds__(256) void narrow_kernel(Product p, bool by_row) {
   }
 }
 
-// float32 dweight with few outputs: dw[g, n, f] for 16 * NF outputs.  A lane
-// takes 4 columns f = 4 * (lane & 15) + e of the row (lane >> 4) * 4 + i, which
-// are four fragments' values at once.  KW of the 4 waves share the rows, the
-// others lie along f.
-template <int NF, int KW>
+// float32 dweight with few outputs: dw[g, n, f] for 16 outputs.  A lane takes 4
+// columns f = 4 * (lane & 15) + e of the row (lane >> 4) * 4 + i, which are four
+// fragments' values at once.  KW of the 4 waves share the rows, the others lie
+// along f.  Bound by reading the rows: 400000 x 256 with 3 outputs in 512
+// groups take 86 us (4.8 TB/s; 64^2 tiles 171).
+template <int KW>
 __global__ __launch_bounds__(256) void narrow_dweight_kernel(Product p) {
   constexpr int BF = 4 / KW * 64;
   const Segment seg = find_segment(p.offsets, p.G, p.C, blockIdx.x, p.shift);
@@ -1604,30 +1605,23 @@ __global__ __launch_bounds__(256) void narrow_dweight_kernel(Product p) {
   const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
   const int part = wave % KW;
   const int f = blockIdx.y * BF + wave / KW * 64 + r * 4;
-  const int n0 = blockIdx.z * NF * 16;
   const int left = p.N - f;
   const bool sums = p.sums && blockIdx.y == 0 && wave / KW == 0;
   const float* a = reinterpret_cast<const float*>(p.a);
   const float* b = reinterpret_cast<const float*>(p.b) + f;
-  int n[NF];
-#pragma unroll
-  for (int j = 0; j < NF; ++j) n[j] = min(n0 + j * 16 + r, p.M - 1);
-  f32x4 acc[NF][4] = {};
-  f32x4 sum[NF] = {};
+  const int n = min(r, p.M - 1);
+  f32x4 acc[4] = {}, sum = {};
 #pragma unroll 2
   for (int s = seg.first + part * 16; s < end; s += KW * 16) {
-    float fa[NF][4];
+    float fa[4];
     f32x4 fb[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int row = s + q * 4 + i;
       const bool in = row < end;
       const long at = in ? row : end - 1;
-#pragma unroll
-      for (int j = 0; j < NF; ++j) {
-        const float v = a[at * p.a_pitch + n[j]];
-        fa[j][i] = in ? v : 0.f;
-      }
+      const float d = a[at * p.a_pitch + n];
+      fa[i] = in ? d : 0.f;
       f32x4 v = {};
       if (left >= 4) {
         __builtin_memcpy(&v, b + at * p.b_pitch, 16);
@@ -1640,37 +1634,28 @@ __global__ __launch_bounds__(256) void narrow_dweight_kernel(Product p) {
       for (int e = 0; e < 4; ++e) fb[i][e] = in ? v[e] : 0.f;
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < 4; ++i) {
 #pragma unroll
-      for (int j = 0; j < NF; ++j) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          acc[j][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(
-              fa[j][i], fb[i][e], acc[j][e], 0, 0, 0);
-        if (sums)
-          sum[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(fa[j][i], 1.f, sum[j],
-                                                        0, 0, 0);
-      }
+      for (int e = 0; e < 4; ++e)
+        acc[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(fa[i], fb[i][e], acc[e],
+                                                      0, 0, 0);
+      if (sums)
+        sum = __builtin_amdgcn_mfma_f32_16x16x4f32(fa[i], 1.f, sum, 0, 0, 0);
+    }
   }
   if constexpr (KW > 1) {
-    __shared__ f32x4 all[4][NF * 5][64];
+    __shared__ f32x4 all[4][5][64];
 #pragma unroll
-    for (int j = 0; j < NF; ++j) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) all[wave][j * 5 + e][lane] = acc[j][e];
-      all[wave][j * 5 + 4][lane] = sum[j];
-    }
+    for (int e = 0; e < 4; ++e) all[wave][e][lane] = acc[e];
+    all[wave][4][lane] = sum;
     __syncthreads();
     if (part) return;
 #pragma unroll
-    for (int w = 1; w < KW; ++w)
+    for (int w = 1; w < KW; ++w) {
 #pragma unroll
-      for (int j = 0; j < NF; ++j) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          acc[j][e] += all[wave + w][j * 5 + e][lane];
-        sum[j] += all[wave + w][j * 5 + 4][lane];
-      }
+      for (int e = 0; e < 4; ++e) acc[e] += all[wave + w][e][lane];
+      sum += all[wave + w][4][lane];
+    }
   }
   const long out_row =
       (parted ? part_place(seg.start, p.shift) +
@@ -1680,17 +1665,69 @@ __global__ __launch_bounds__(256) void narrow_dweight_kernel(Product p) {
   float* out = parted && p.out ? p.part : reinterpret_cast<float*>(p.out);
   float* out_sums = parted ? p.part_sums : reinterpret_cast<float*>(p.sums);
 #pragma unroll
-  for (int j = 0; j < NF; ++j)
+  for (int i = 0; i < 4; ++i) {
+    const int m = q * 4 + i;
+    if (m >= p.M) continue;
+    float* to = out + (out_row + m) * p.N + f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int m = n0 + j * 16 + q * 4 + i;
-      if (m >= p.M) continue;
-      float* to = out + (out_row + m) * p.N + f;
+    for (int e = 0; e < 4; ++e)
+      if (p.out && e < left) to[e] = acc[e][i];
+    if (sums && r == 0) out_sums[out_row + m] = sum[i];
+  }
+}
+
+// drows with a short contraction (the classes of a keyed model, C <= NB):
+// bound by writing the rows.  A lane holds its columns' weights, the rows' dy
+// are in LDS in 32 bits, and a wave writes 32 rows in whole vectors; `lanes`
+// lanes (a power of two) share a row.
+template <typename T, int NB>
+__global__ __launch_bounds__(256) void narrow_drows_kernel(Product p,
+                                                           int lanes) {
+  constexpr int V = 16 / sizeof(T), BM = 128;
+  const Segment seg =
+      find_segment(p.offsets, p.G, p.M, blockIdx.x, log2_of(BM));
+  if (seg.first >= seg.end) return;
+  __shared__ __align__(16) float d[BM][NB];
+  const int rows = min(BM, seg.end - seg.first);
+  const bool any = seg.group < p.G;
+  const T* a = reinterpret_cast<const T*>(p.a) + seg.first * p.a_pitch;
+  for (int i = threadIdx.x; i < BM * NB; i += 256) {
+    const int row = i / NB, n = i % NB;
+    d[row][n] = any && row < rows && n < p.C ? to_f(a[row * p.a_pitch + n])
+                                             : 0.f;
+  }
+  __syncthreads();
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int per = 64 / lanes;
+  const int end = min(rows, wave * 32 + 32);
+  const T* b = reinterpret_cast<const T*>(p.b) +
+               (long)min(seg.group, p.G - 1) * p.C * p.N;
+  T* out = reinterpret_cast<T*>(p.out) + (long)seg.first * p.N;
+  for (int f = (blockIdx.y * lanes + lane % lanes) * V; f < p.N;
+       f += gridDim.y * lanes * V) {
+    const int left = p.N - f;
+    float w[NB][V];
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (p.out && e < left) to[e] = acc[j][e][i];
-      if (sums && r == 0) out_sums[out_row + m] = sum[j][i];
+    for (int n = 0; n < NB; ++n) {
+      Vec<T> v = {};
+      if (any && n < p.C) v = load_vec(b + (long)n * p.N + f, left);
+#pragma unroll
+      for (int i = 0; i < V; ++i) w[n][i] = to_f(v.v[i]);
     }
+    for (int row = wave * 32 + lane / lanes; row < end; row += per) {
+      float acc[V] = {};
+#pragma unroll
+      for (int n = 0; n < NB; ++n) {
+        const float x = d[row][n];
+#pragma unroll
+        for (int i = 0; i < V; ++i) acc[i] += x * w[n][i];
+      }
+      Vec<T> v;
+#pragma unroll
+      for (int i = 0; i < V; ++i) v.v[i] = (T)acc[i];
+      store_vec(out + (long)row * p.N + f, v, left);
+    }
+  }
 }
 
 // Buffer loads to LDS take addresses of whole words.
@@ -1716,10 +1753,28 @@ bool narrow_launch(const Product& p) {
     check_launch();
     return true;
   };
-  if (rows <= 16) return go(narrow_kernel<T, 1, 1, 4>, 16, 16);
-  if (p.N <= 16) return go(narrow_kernel<T, 4, 1, 1>, 256, 16);
-  if (p.N <= 32) return go(narrow_kernel<T, 4, 2, 1>, 256, 32);
-  if (p.N <= 64) return go(narrow_kernel<T, 4, 4, 1>, 256, 64);
+  // Measured against the tile kernels, us (type, rows, groups, outputs,
+  // columns; the kernels by rows x outputs of a wave, k: its share of c):
+  //   float32       8,   64, 2048, 2048: 16 x 32 k 34, tiles  83
+  //   float32    2000,  200,  512,  512: 16 x 32 k 45, tiles  69
+  //   float32    3000,   64, 1024, 1024: 16 x 32 k 203, tiles 110
+  //   bfloat16      8,   64, 2048, 2048: 16 x 16 k 12, tiles  20
+  //   bfloat16   2000,  200,  512,  512: 16 x 16 k 28, tiles  22
+  //   float32 1000000, 1000,  10,  256: 64 x 16 225, 32 x 16 k 247, tiles 355
+  //   float32  200000, 1000,   3,  250: 64 x 16  56, 32 x 16 k  42, tiles  88
+  //   float32  400000, 1000,  32,  256: 32 x 32 127, tiles 149
+  //   float32  400000, 1000,  64,  256: 32 x 32 244, tiles 164
+  //   bfloat16 200000, 1000,   3,  250: 64 x 16  31, 32 x 16 k  23, tiles  35
+  //   bfloat16 400000, 1000,  32,  256: 64 x 32  51, tiles  49
+  constexpr bool kWide = sizeof(T) == 4;
+  if (rows <= (kWide ? 16 : 8))
+    return kWide ? go(narrow_kernel<T, 1, 2, 4>, 16, 32)
+                 : go(narrow_kernel<T, 1, 1, 4>, 16, 16);
+  if (p.N <= 16)
+    return rows >= 512 && p.C < 512 ? go(narrow_kernel<T, 4, 1, 1>, 256, 16)
+                                    : go(narrow_kernel<T, 2, 1, 4>, 32, 16);
+  if constexpr (kWide)
+    if (p.N <= 32) return go(narrow_kernel<T, 2, 2, 1>, 128, 32);
   return false;
 }
 
@@ -1850,23 +1905,37 @@ void product_launch(Product p, at::TensorOptions opt) {
 
 void narrow_dweight_launch(Product p, at::TensorOptions opt) {
   const int kw = p.N <= 64 ? 4 : 1, bf = 4 / kw * 64;
-  const int nf = p.M <= 16 ? 1 : 2;
-  const long n_tiles =
-      ((p.M + nf * 16 - 1) / (nf * 16)) * (long)((p.N + bf - 1) / bf);
-  p.shift = part_shift(p.C, n_tiles, 2048);
+  const long tiles = (p.N + bf - 1) / bf;
+  p.shift = part_shift(p.C, tiles, 2048);
   Parts parts = take_parts(p, opt);
-  dim3 grid(grid_of(((long)p.C >> p.shift) + p.G + 1, 256),
-            p.out ? (p.N + bf - 1) / bf : 1, (p.M + nf * 16 - 1) / (nf * 16));
-  TORCH_CHECK(grid.y < 65536 && grid.z < 65536, "rows are too wide");
+  dim3 grid(grid_of(((long)p.C >> p.shift) + p.G + 1, 256), p.out ? tiles : 1);
+  TORCH_CHECK(grid.y < 65536, "rows are too wide");
+  if (kw == 4)
+    narrow_dweight_kernel<4><<<grid, 256, 0, stream_now()>>>(p);
+  else
+    narrow_dweight_kernel<1><<<grid, 256, 0, stream_now()>>>(p);
+  check_launch();
+  finish_launch<float>(p);
+}
+
+template <typename T>
+void narrow_drows_launch(const Product& p) {
+  const int lanes = lanes_for(p.N, 16 / sizeof(T));
+  const long blocks = (long)p.M / 128 + p.G + 1;
+  // the columns are shared among blocks where there are few row tiles
+  const long parts = (p.N * sizeof(T) + 16 * lanes - 1) / (16 * lanes);
+  dim3 grid(grid_of(blocks, 256),
+            std::max(1l, std::min({parts, 2048 / blocks, 1024l})));
   auto go = [&](auto kern) {
-    kern<<<grid, 256, 0, stream_now()>>>(p);
+    kern<<<grid, 256, 0, stream_now()>>>(p, lanes);
     check_launch();
   };
-  if (kw == 4)
-    nf == 1 ? go(narrow_dweight_kernel<1, 4>) : go(narrow_dweight_kernel<2, 4>);
+  if (p.C <= 4)
+    go(narrow_drows_kernel<T, 4>);
+  else if (p.C <= 8)
+    go(narrow_drows_kernel<T, 8>);
   else
-    nf == 1 ? go(narrow_dweight_kernel<1, 1>) : go(narrow_dweight_kernel<2, 1>);
-  finish_launch<float>(p);
+    go(narrow_drows_kernel<T, 16>);
 }
 
 at::Tensor product(const at::Tensor& a_in, const at::Tensor& weight,
@@ -1885,7 +1954,9 @@ at::Tensor product(const at::Tensor& a_in, const at::Tensor& weight,
             offsets.data_ptr<int>(), a.stride(0), transposed ? N : C, G, M, N,
             C, 0, nullptr, nullptr, 0};
   SKA_TYPES(a.scalar_type(), [&] {
-    if (transposed)
+    if (transposed && C <= 16)
+      narrow_drows_launch<T>(p);
+    else if (transposed)
       product_launch<T, kDRows>(p, a.options());
     else
       product_launch<T, kForward>(p, a.options());
@@ -1932,7 +2003,7 @@ grouped_linear_dweight(const at::Tensor& dy_in, const at::Tensor& rows_in,
             offsets.data_ptr<int>(), dy.stride(0), b.stride(0), G, N,
             F ? F : N, M, 0, nullptr, nullptr, 0};
   SKA_TYPES(dy.scalar_type(), [&] {
-    if (sizeof(T) == 4 && N <= 64)
+    if (sizeof(T) == 4 && N <= 16)
       narrow_dweight_launch(p, dy.options());
     else
       product_launch<T, kDWeight>(p, dy.options());
