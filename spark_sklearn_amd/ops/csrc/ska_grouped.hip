@@ -57,7 +57,8 @@ __device__ __forceinline__ int key_of(I id, int G) {
 }
 
 // The first position in keys[0, n) whose key is not below g.
-__device__ __forceinline__ int lower_bound(const int* keys, int n, int g) {
+template <typename K>
+__device__ __forceinline__ int lower_bound(const K* keys, int n, K g) {
   int lo = 0, hi = n;
   while (lo < hi) {
     int mid = (lo + hi) >> 1;
@@ -72,37 +73,55 @@ __device__ __forceinline__ int lower_bound(const int* keys, int n, int g) {
 constexpr int kSmallEntries = 2048;
 constexpr int kSmallGroups = 65536;
 
-// Few entries: one block.  An entry's slot is the number of entries that go
-// before it, counted by comparing it with every other, four keys a read.
+// LDS accesses before and after it keep their order within the wave.
+__device__ __forceinline__ void wave_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// Few entries: one block sorts key * 2048 + entry, which makes the order
+// stable, in LDS: compare and exchange at distances of halves.  Distances
+// below 64 stay within a wave, where no barrier is needed.  2012 entries took
+// 158 us by comparing each with every other.
 template <typename I>
 __global__ __launch_bounds__(1024) void sort_small_kernel(
-    const I* __restrict__ ids, int M, int G, int* __restrict__ offsets,
-    int* __restrict__ slots, int* __restrict__ order) {
-  __shared__ int4 key4[kSmallEntries / 4];
-  __shared__ int sorted[kSmallEntries];
-  int* key = reinterpret_cast<int*>(key4);
-  const int tid = threadIdx.x;
-  const int M4 = (M + 3) >> 2;
-  for (int i = tid; i < M4 * 4; i += 1024)
-    key[i] = i < M ? key_of<I>(ids[i], G) : 0x7fffffff;
+    const I* __restrict__ ids, int M, int G, int size,
+    int* __restrict__ offsets, int* __restrict__ slots,
+    int* __restrict__ order) {
+  static_assert((kSmallGroups + 1l) * kSmallEntries < (1l << 32));
+  __shared__ unsigned item[kSmallEntries];
+  const int tid = threadIdx.x, threads = blockDim.x;
+  for (int i = tid; i < size; i += threads)
+    item[i] = i < M ? (unsigned)key_of<I>(ids[i], G) * kSmallEntries + i
+                    : 0xffffffffu;
   __syncthreads();
-  for (int i = tid; i < M; i += 1024) {
-    const int me = key[i];
-    int before = 0;
-    for (int q = 0; q < M4; ++q) {
-      const int4 v = key4[q];
-      const int j = q * 4;
-      before += (v.x < me || (v.x == me && j < i));
-      before += (v.y < me || (v.y == me && j + 1 < i));
-      before += (v.z < me || (v.z == me && j + 2 < i));
-      before += (v.w < me || (v.w == me && j + 3 < i));
+  for (int run = 2; run <= size; run *= 2)
+    for (int d = run / 2; d > 0; d /= 2) {
+      for (int t = tid; t < size / 2; t += threads) {
+        // the pair of elements d apart that thread t owns
+        const int a = (t & -d) * 2 + (t & (d - 1)), b = a + d;
+        const unsigned x = item[a], y = item[b];
+        const bool up = (a & run) == 0;
+        if ((x > y) == up) {
+          item[a] = y;
+          item[b] = x;
+        }
+      }
+      // 64 threads own 128 neighbouring elements while d < 64
+      if (d > 64 || (d == 1 && run >= 64))
+        __syncthreads();
+      else
+        wave_fence();
     }
-    slots[i] = before;
-    order[before] = i;
-    sorted[before] = me;
-  }
   __syncthreads();
-  for (int g = tid; g <= G; g += 1024) offsets[g] = lower_bound(sorted, M, g);
+  for (int i = tid; i < M; i += threads) {
+    const int entry = item[i] & (kSmallEntries - 1);
+    order[i] = entry;
+    slots[entry] = i;
+  }
+  for (int g = tid; g <= G; g += threads)
+    offsets[g] = lower_bound(item, M, (unsigned)g * kSmallEntries);
 }
 
 // Many entries: passes over a digit of the key, low digit first.  One pass
@@ -265,7 +284,10 @@ void sort_launch(const I* ids, int M, int G, int* offsets, int* slots,
                  int* order, at::TensorOptions opt) {
   hipStream_t s = stream_now();
   if (M <= kSmallEntries && G <= kSmallGroups) {
-    sort_small_kernel<I><<<1, 1024, 0, s>>>(ids, M, G, offsets, slots, order);
+    int size = 2;
+    while (size < M) size *= 2;
+    sort_small_kernel<I><<<1, std::min(1024, std::max(64, size / 2)), 0, s>>>(
+        ids, M, G, size, offsets, slots, order);
     check_launch();
     return;
   }
@@ -828,37 +850,42 @@ __device__ __forceinline__ int edge(const int* offsets, int g, int G, int M) {
   return g <= 0 ? 0 : (g > G ? M : clampi(offsets[g], 0, M));
 }
 
-// The last group g with floor(offsets[g] >> shift) + g * each <= at.  Each
-// round, 64 lanes look at 64 evenly spaced groups: 4095 groups take two.
-__device__ __forceinline__ int find_group(const int* offsets, int G, int M,
-                                          int at, int shift, int each) {
+// The last group g with floor(offsets[g] >> shift) + g * each <= at, and its
+// rows.  Each round, the lanes look at evenly spaced groups; the last round
+// has the group's own edges at hand, so that 62 groups take one read and 3906
+// take two.
+struct Group {
+  int g, start, end;
+};
+
+__device__ __forceinline__ Group find_group(const int* offsets, int G, int M,
+                                            int at, int shift, int each) {
   const int lane = threadIdx.x & 63;
-  int lo = 0, n = G + 1;
-  while (n > 1) {
-    const int step = (n + 63) >> 6;
+  int lo = 0, n = G + 1;  // the groups lo .. lo + n - 1 are left
+  while (true) {
+    const int step = (n + 62) / 63;
     const int g = lo + lane * step;
-    const bool in =
-        lane * step < n && (edge(offsets, g, G, M) >> shift) + g * each <= at;
+    const int e = edge(offsets, min(g, G + 1), G, M);
+    const bool in = lane * step < n && (e >> shift) + g * each <= at;
     // offsets do not decrease, so these are the lanes up to some lane; lane 0
     // counts in any case
     const unsigned long long set = __ballot(in) | 1ull;
     const int last = 63 - __builtin_clzll(set);
+    if (step == 1)
+      return {__builtin_amdgcn_readfirstlane(lo + last),
+              __builtin_amdgcn_readlane(e, last),
+              __builtin_amdgcn_readlane(e, last + 1)};
     lo += last * step;
     n = min(step, n - last * step);
   }
-  return __builtin_amdgcn_readfirstlane(lo);
 }
 
 __device__ __forceinline__ Segment find_segment(const int* offsets, int G,
                                                 int M, int tile, int shift) {
-  const int g = find_group(offsets, G, M, tile, shift, 1);
-  const int start = edge(offsets, g, G, M);
-  const int end = edge(offsets, g + 1, G, M);
+  const Group of = find_group(offsets, G, M, tile, shift, 1);
   const long first =
-      start + ((long)(tile - ((start >> shift) + g)) << shift);
-  return {g, __builtin_amdgcn_readfirstlane(start),
-          __builtin_amdgcn_readfirstlane((int)min(first, (long)end)),
-          __builtin_amdgcn_readfirstlane(end)};
+      of.start + ((long)(tile - ((of.start >> shift) + of.g)) << shift);
+  return {of.g, of.start, (int)min(first, (long)of.end), of.end};
 }
 
 // Where a part of a group's rows leaves its sums.  A group of n > R = 2^shift
@@ -873,13 +900,9 @@ __device__ __forceinline__ long part_place(int start, int shift) {
 __device__ __forceinline__ Segment find_segment_at(const int* offsets, int G,
                                                    int M, int row,
                                                    int shift) {
-  const int g = find_group(offsets, G, M, row, 0, 0);
-  const int start = edge(offsets, g, G, M);
-  const int end = edge(offsets, g + 1, G, M);
-  const bool head = ((row - start) & ((1 << shift) - 1)) == 0;
-  return {g, __builtin_amdgcn_readfirstlane(start),
-          __builtin_amdgcn_readfirstlane(head ? row : end),
-          __builtin_amdgcn_readfirstlane(end)};
+  const Group of = find_group(offsets, G, M, row, 0, 0);
+  const bool head = ((row - of.start) & ((1 << shift) - 1)) == 0;
+  return {of.g, of.start, head ? row : of.end, of.end};
 }
 
 __host__ __device__ constexpr int log2_of(int v) {
@@ -1115,10 +1138,9 @@ struct Tile {
   }
 };
 
-// Waits until at most N loads are under way.
-template <int N>
+// Waits for a wave's own loads.
 __device__ __forceinline__ void wait_loads() {
-  __builtin_amdgcn_s_waitcnt(0x0f70 | (N & 15) | ((N >> 4) << 14));
+  __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0), nothing else
 }
 
 // A barrier for what the block wrote to LDS itself; loads under way go on.
@@ -1226,17 +1248,16 @@ __device__ __forceinline__ bool find_job(const Product& p, int tile,
   return true;
 }
 
-// STAGES tiles of c in LDS (0: two, filled through registers).
-template <typename T, int BM, int BN, int WM, int WN, int MODE, int STAGES>
+// Two tiles of c in LDS, filled by loads that write it (ASYNC) or through
+// registers.
+template <typename T, int BM, int BN, int WM, int WN, int MODE, bool ASYNC>
 __global__ __launch_bounds__(WM* WN * 64) void product_kernel(Product p) {
   constexpr int kThreads = WM * WN * 64;
   constexpr int FM = BM / WM / 16, FN = BN / WN / 16;
   typedef Tile<T, BM, MODE == kDWeight, kThreads, 1> TA;
   typedef Tile<T, BN, MODE != kForward, kThreads, FN> TB;
   constexpr int KS = TA::KS;
-  constexpr bool ASYNC = STAGES > 0;
-  constexpr int kBuffers = ASYNC ? STAGES : 2;
-  __shared__ __align__(16) char lds[kBuffers][TA::kBytes + TB::kBytes];
+  __shared__ __align__(16) char lds[2][TA::kBytes + TB::kBytes];
 
   // Blocks go round the 8 XCDs: each XCD gets a contiguous run of tiles, whose
   // operands its L2 then holds.
@@ -1269,7 +1290,6 @@ __global__ __launch_bounds__(WM* WN * 64) void product_kernel(Product p) {
         job.steps - c};
   };
   constexpr int kLoads = TA::kPer + TB::kPer;
-  constexpr int kAhead = ASYNC ? STAGES - 1 : 1;
   Vec<T> ra[ASYNC ? 1 : TA::kPer], rb[ASYNC ? 1 : TB::kPer];
   auto load = [&](const Source& s, int buf, int i) {
     if (i < TA::kPer)
@@ -1295,12 +1315,9 @@ __global__ __launch_bounds__(WM* WN * 64) void product_kernel(Product p) {
 
   if (job.steps > 0) {
     if constexpr (ASYNC) {
+      const Source from = source(0);
 #pragma unroll
-      for (int s = 0; s < kAhead; ++s) {
-        const Source from = source(s * KS);
-#pragma unroll
-        for (int i = 0; i < kLoads; ++i) load(from, s, i);
-      }
+      for (int i = 0; i < kLoads; ++i) load(from, 0, i);
     } else {
       load_regs(source(0));
     }
@@ -1309,9 +1326,9 @@ __global__ __launch_bounds__(WM* WN * 64) void product_kernel(Product p) {
 #pragma unroll 1
   for (int c = 0; c < job.steps; c += KS) {
     // Tile c lands.  At the barrier all waves have also read the tile
-    // before, whose place the loads of the tile kAhead further then take.
+    // before, whose place the loads of the next then take.
     if constexpr (ASYNC) {
-      wait_loads<kLoads*(kAhead - 1)>();
+      wait_loads();
       const Source s = source(c);
       if (s.ba.ragged)
         TA::fill(s.a, p.a_pitch, job.rows, s.steps, s.ba, lds[buf]);
@@ -1324,9 +1341,7 @@ __global__ __launch_bounds__(WM* WN * 64) void product_kernel(Product p) {
     }
     block_barrier();
     // Behind the last tile of all these loads write zeros, for nobody.
-    const Source next = source(c + kAhead * KS);
-    const int to = buf + kAhead >= kBuffers ? buf + kAhead - kBuffers
-                                            : buf + kAhead;
+    const Source next = source(c + KS);
     if constexpr (!ASYNC)
       if (next.steps > 0) load_regs(next);
     const char* la = lds[buf];
@@ -1351,7 +1366,7 @@ __global__ __launch_bounds__(WM* WN * 64) void product_kernel(Product p) {
         if constexpr (ASYNC) {
 #pragma unroll
           for (int l = i * kLoads / FM; l < (i + 1) * kLoads / FM; ++l)
-            load(next, to, l);
+            load(next, buf ^ 1, l);
         }
       }
 #pragma unroll
@@ -1361,11 +1376,11 @@ __global__ __launch_bounds__(WM* WN * 64) void product_kernel(Product p) {
         sum[i % FS] = Mma<T>::go(ones, fa[g & 1], sum[i % FS]);
       __builtin_amdgcn_sched_barrier(0);
     }
-    buf = buf + 1 == kBuffers ? 0 : buf + 1;
+    buf ^= 1;
   }
 
   // LDS is not given back with loads under way.
-  if constexpr (ASYNC) wait_loads<0>();
+  if constexpr (ASYNC) wait_loads();
 
   // lane: row m = lane & 15 of each fragment, 4 * FN neighbouring columns
   T* out = reinterpret_cast<T*>(p.out);
@@ -1815,10 +1830,12 @@ void finish_launch(const Product& p) {
 template <typename T, int MODE>
 void product_launch(Product p, at::TensorOptions opt) {
   if (MODE == kForward && narrow_launch<T>(p)) return;
-  const bool async = whole_words((const T*)p.a, p.a_pitch) &&
-                     whole_words((const T*)p.b, p.b_pitch) &&
-                     // the weights of a group may begin at an odd value
-                     (MODE == kDWeight || ((long)p.N * p.C) % 2 == 0);
+  const bool async =
+      sizeof(T) == 4 ||
+      (whole_words((const T*)p.a, p.a_pitch) &&
+       whole_words((const T*)p.b, p.b_pitch) &&
+       // the weights of a group may begin at an odd value
+       (MODE == kDWeight || ((long)p.N * p.C) % 2 == 0));
   auto tiles = [&](long b) { return (p.M + b - 1) / b * ((p.N + b - 1) / b); };
   auto go = [&](auto kern, int bm, int bn, int threads) {
     const long m_tiles = (p.M + bm - 1) / bm;
@@ -1844,35 +1861,34 @@ void product_launch(Product p, at::TensorOptions opt) {
   // waste less of the groups' last tiles and leave more blocks to hide the
   // loads behind.  Measured on bfloat16, us for 256^2 / 128^2 / 64 x 128 /
   // 64^2 tiles (rows, groups, outputs, columns):
-  //   forward  65536, 32, 4096, 1024:  685 / 788 / 1178 / 1195
-  //            16384, 64, 1024, 1024:   64 /  57 /   68 /   75
-  //             8198, 48,  768,  768:   28 /  28 /   24 /   26
-  //             8192,  8,  256,  256:   12 /   7 /    7 /    6
-  //   dweight  65536, 32, 4096, 1024:  747 / 931 / 1511 / 1447
-  //             8198, 48,  768,  768:   36 /  33 /   49 /   47
-  //            65536, 256,  64,  256:   46 /  34 /   31 /   24
+  //   forward  65536, 32, 4096, 1024:  625 / 754 /  879 / 1018
+  //            14420, 132, 3330, 904:  300 / 284 /  325 /  374
+  //            16384, 64, 1024, 1024:   57 /  58 /   62 /   76
+  //             8198, 48,  768,  768:   25 /  28 /   25 /   27
+  //             3000, 64, 1024, 1024:   53 /  37 /   26 /   32
+  //             8192,  8,  256,  256:   12 /   8 /    8 /    7
+  //   dweight  65536, 32, 4096, 1024:  693 / 959 / 1324 / 1397
+  //            65536, 64,  256, 1024:   99 /  78 /   70 /   79
+  //            28273, 179, 2072,  84:   84 /  59 /   59 /   61
+  //            60000, 300,  720,  40:   60 /  45 /   42 /   31
+  constexpr bool kWide = sizeof(T) == 4;  // float32 has no larger ones
   if (MODE == kDWeight) {
-    // 256^2 where that fills the card and its edges waste less than a third
-    const bool large = p.G * tiles(256) >= 192 &&
+    // 256^2 where that fills the card twice and its edges waste less than a
+    // third
+    const bool large = p.G * tiles(256) >= 512 &&
                        tiles(256) * 65536 * 3 <= 4l * p.M * p.N;
     const bool middle = p.M > 64 && p.N > 64 && p.G * tiles(128) >= 256;
-    if constexpr (sizeof(T) == 4) {
-      if (middle)
-        go(product_kernel<T, 128, 128, 2, 2, MODE, 2>, 128, 128, 256);
-      else
-        go(product_kernel<T, 64, 64, 2, 2, MODE, 3>, 64, 64, 256);
-      return;
+    if (large && async && !kWide) {
+      if constexpr (!kWide)
+        go(product_kernel<T, 256, 256, 2, 4, MODE, true>, 256, 256, 512);
+    } else if (large || middle) {
+      async ? go(product_kernel<T, 128, 128, 2, 2, MODE, true>, 128, 128, 256)
+            : go(product_kernel<T, 128, 128, 2, 2, MODE, kWide>, 128, 128,
+                 256);
+    } else {
+      async ? go(product_kernel<T, 64, 64, 2, 2, MODE, true>, 64, 64, 256)
+            : go(product_kernel<T, 64, 64, 2, 2, MODE, kWide>, 64, 64, 256);
     }
-    if (async && large)
-      go(product_kernel<T, 256, 256, 2, 4, MODE, 2>, 256, 256, 512);
-    else if (async && middle)
-      go(product_kernel<T, 128, 128, 2, 2, MODE, 2>, 128, 128, 256);
-    else if (async)
-      go(product_kernel<T, 64, 64, 2, 2, MODE, 3>, 64, 64, 256);
-    else if (large || middle)
-      go(product_kernel<T, 128, 128, 2, 2, MODE, 0>, 128, 128, 256);
-    else
-      go(product_kernel<T, 64, 64, 2, 2, MODE, 0>, 64, 64, 256);
     return;
   }
   const long each = p.M / std::min(p.G, p.M);  // rows a group
@@ -1880,27 +1896,21 @@ void product_launch(Product p, at::TensorOptions opt) {
     return (p.M / bm + std::min(p.G, p.M) / 2 + 1) * ((p.N + bn - 1) / bn);
   };
   const bool large = each >= 768 && p.N > 128 && row_tiles(256, 256) >= 512;
-  const bool middle = each >= 192 && p.N > 64 && row_tiles(128, 128) >= 256;
-  if constexpr (sizeof(T) == 4) {
-    // 128^2 tiles reach the matrix units' rate in float32
-    if (p.N > 64 && each >= 64 && row_tiles(128, 128) >= 256)
-      go(product_kernel<T, 128, 128, 2, 2, MODE, 2>, 128, 128, 256);
-    else
-      go(product_kernel<T, 64, 64, 2, 2, MODE, 3>, 64, 64, 256);
-    return;
+  const bool middle =
+      p.N > 64 && ((each >= 192 && row_tiles(128, 128) >= 256) ||
+                   (each >= 96 && row_tiles(128, 128) >= 1024));
+  if (large && async && !kWide) {
+    if constexpr (!kWide)
+      go(product_kernel<T, 256, 256, 2, 4, MODE, true>, 256, 256, 512);
+  } else if (large || middle) {
+    async ? go(product_kernel<T, 128, 128, 2, 2, MODE, true>, 128, 128, 256)
+          : go(product_kernel<T, 128, 128, 2, 2, MODE, kWide>, 128, 128, 256);
+  } else if (async && p.N > 64 && row_tiles(64, 128) >= 256) {
+    go(product_kernel<T, 64, 128, 1, 4, MODE, true>, 64, 128, 256);
+  } else {
+    async ? go(product_kernel<T, 64, 64, 2, 2, MODE, true>, 64, 64, 256)
+          : go(product_kernel<T, 64, 64, 2, 2, MODE, kWide>, 64, 64, 256);
   }
-  if (async && large)
-    go(product_kernel<T, 256, 256, 2, 4, MODE, 2>, 256, 256, 512);
-  else if (async && middle)
-    go(product_kernel<T, 128, 128, 2, 2, MODE, 2>, 128, 128, 256);
-  else if (async && p.N > 64 && row_tiles(64, 128) >= 256)
-    go(product_kernel<T, 64, 128, 1, 4, MODE, 3>, 64, 128, 256);
-  else if (async)
-    go(product_kernel<T, 64, 64, 2, 2, MODE, 3>, 64, 64, 256);
-  else if (large || middle)
-    go(product_kernel<T, 128, 128, 2, 2, MODE, 0>, 128, 128, 256);
-  else
-    go(product_kernel<T, 64, 64, 2, 2, MODE, 0>, 64, 64, 256);
 }
 
 void narrow_dweight_launch(Product p, at::TensorOptions opt) {
