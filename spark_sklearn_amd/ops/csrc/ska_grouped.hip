@@ -1248,16 +1248,19 @@ __device__ __forceinline__ bool find_job(const Product& p, int tile,
   return true;
 }
 
-// Two tiles of c in LDS, filled by loads that write it (ASYNC) or through
-// registers.
-template <typename T, int BM, int BN, int WM, int WN, int MODE, bool ASYNC>
+// Tiles of c in LDS, filled by loads that write it (ASYNC) or through
+// registers: two, or one (not AHEAD) for short contractions, whose blocks hide
+// each other's loads and of which more then fit a CU.
+template <typename T, int BM, int BN, int WM, int WN, int MODE, bool ASYNC,
+          bool AHEAD = true>
 __global__ __launch_bounds__(WM* WN * 64) void product_kernel(Product p) {
   constexpr int kThreads = WM * WN * 64;
   constexpr int FM = BM / WM / 16, FN = BN / WN / 16;
   typedef Tile<T, BM, MODE == kDWeight, kThreads, 1> TA;
   typedef Tile<T, BN, MODE != kForward, kThreads, FN> TB;
   constexpr int KS = TA::KS;
-  __shared__ __align__(16) char lds[2][TA::kBytes + TB::kBytes];
+  static_assert(ASYNC || AHEAD);
+  __shared__ __align__(16) char lds[AHEAD ? 2 : 1][TA::kBytes + TB::kBytes];
 
   // Blocks go round the 8 XCDs: each XCD gets a contiguous run of tiles, whose
   // operands its L2 then holds.
@@ -1340,7 +1343,7 @@ __global__ __launch_bounds__(WM* WN * 64) void product_kernel(Product p) {
       TB::store_regs(rb, lds[buf] + TA::kBytes);
     }
     block_barrier();
-    // Behind the last tile of all these loads write zeros, for nobody.
+    // Behind the last tile these loads write zeros, for nobody.
     const Source next = source(c + KS);
     if constexpr (!ASYNC)
       if (next.steps > 0) load_regs(next);
@@ -1363,7 +1366,7 @@ __global__ __launch_bounds__(WM* WN * 64) void product_kernel(Product p) {
 #pragma unroll
         for (int j = i * FN / FM; j < (i + 1) * FN / FM; ++j)
           fb[1][j] = TB::frag(lb, wn, j, 1);
-        if constexpr (ASYNC) {
+        if constexpr (ASYNC && AHEAD) {
 #pragma unroll
           for (int l = i * kLoads / FM; l < (i + 1) * kLoads / FM; ++l)
             load(next, buf ^ 1, l);
@@ -1376,7 +1379,13 @@ __global__ __launch_bounds__(WM* WN * 64) void product_kernel(Product p) {
         sum[i % FS] = Mma<T>::go(ones, fa[g & 1], sum[i % FS]);
       __builtin_amdgcn_sched_barrier(0);
     }
-    buf ^= 1;
+    if constexpr (AHEAD) {
+      buf ^= 1;
+    } else if (next.steps > 0) {
+      block_barrier();
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) load(next, 0, i);
+    }
   }
 
   // LDS is not given back with loads under way.
@@ -1871,7 +1880,33 @@ void product_launch(Product p, at::TensorOptions opt) {
   //            65536, 64,  256, 1024:   99 /  78 /   70 /   79
   //            28273, 179, 2072,  84:   84 /  59 /   59 /   61
   //            60000, 300,  720,  40:   60 /  45 /   42 /   31
+  //
+  // One tile of c at a time, where enough blocks share a CU (us with two / one
+  // at 128^2): forward 28273, 179, 2072, 84: 93 / 71; 40000, 400, 512, 512:
+  // 64 / 60; but drows 3000, 64, 64, 1024: 16 / 20.
   constexpr bool kWide = sizeof(T) == 4;  // float32 has no larger ones
+  constexpr long KS = 128 / sizeof(T);
+  auto tile128 = [&](bool ahead) {
+    if (!async)
+      go(product_kernel<T, 128, 128, 2, 2, MODE, kWide>, 128, 128, 256);
+    else if (ahead)
+      go(product_kernel<T, 128, 128, 2, 2, MODE, true>, 128, 128, 256);
+    else
+      go(product_kernel<T, 128, 128, 2, 2, MODE, true, false>, 128, 128, 256);
+  };
+  auto tile64 = [&](bool ahead) {
+    if (!async)
+      go(product_kernel<T, 64, 64, 2, 2, MODE, kWide>, 64, 64, 256);
+    else if (ahead)
+      go(product_kernel<T, 64, 64, 2, 2, MODE, true>, 64, 64, 256);
+    else
+      go(product_kernel<T, 64, 64, 2, 2, MODE, true, false>, 64, 64, 256);
+  };
+  const long each =  // rows a group
+      MODE == kDWeight ? p.C / p.G : p.M / std::min(p.G, p.M);
+  auto ahead = [&](long blocks) {
+    return blocks < 1024 && (MODE == kDWeight ? each : p.C) > 2 * KS;
+  };
   if (MODE == kDWeight) {
     // 256^2 where that fills the card twice and its edges waste less than a
     // third
@@ -1882,16 +1917,12 @@ void product_launch(Product p, at::TensorOptions opt) {
       if constexpr (!kWide)
         go(product_kernel<T, 256, 256, 2, 4, MODE, true>, 256, 256, 512);
     } else if (large || middle) {
-      async ? go(product_kernel<T, 128, 128, 2, 2, MODE, true>, 128, 128, 256)
-            : go(product_kernel<T, 128, 128, 2, 2, MODE, kWide>, 128, 128,
-                 256);
+      tile128(ahead(p.G * tiles(128)));
     } else {
-      async ? go(product_kernel<T, 64, 64, 2, 2, MODE, true>, 64, 64, 256)
-            : go(product_kernel<T, 64, 64, 2, 2, MODE, kWide>, 64, 64, 256);
+      tile64(ahead(p.G * tiles(64)));
     }
     return;
   }
-  const long each = p.M / std::min(p.G, p.M);  // rows a group
   auto row_tiles = [&](long bm, long bn) {
     return (p.M / bm + std::min(p.G, p.M) / 2 + 1) * ((p.N + bn - 1) / bn);
   };
@@ -1903,13 +1934,14 @@ void product_launch(Product p, at::TensorOptions opt) {
     if constexpr (!kWide)
       go(product_kernel<T, 256, 256, 2, 4, MODE, true>, 256, 256, 512);
   } else if (large || middle) {
-    async ? go(product_kernel<T, 128, 128, 2, 2, MODE, true>, 128, 128, 256)
-          : go(product_kernel<T, 128, 128, 2, 2, MODE, kWide>, 128, 128, 256);
+    tile128(ahead(row_tiles(128, 128)));
   } else if (async && p.N > 64 && row_tiles(64, 128) >= 256) {
-    go(product_kernel<T, 64, 128, 1, 4, MODE, true>, 64, 128, 256);
+    if (ahead(row_tiles(64, 128)))
+      go(product_kernel<T, 64, 128, 1, 4, MODE, true>, 64, 128, 256);
+    else
+      go(product_kernel<T, 64, 128, 1, 4, MODE, true, false>, 64, 128, 256);
   } else {
-    async ? go(product_kernel<T, 64, 64, 2, 2, MODE, true>, 64, 64, 256)
-          : go(product_kernel<T, 64, 64, 2, 2, MODE, kWide>, 64, 64, 256);
+    tile64(ahead(row_tiles(64, 64)));
   }
 }
 
