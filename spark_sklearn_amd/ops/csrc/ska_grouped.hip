@@ -136,6 +136,26 @@ __device__ __forceinline__ int sort_key(const I* ids, const int* keys, int G,
   return FIRST ? key_of<I>(ids[i], G) : keys[i];
 }
 
+// Keys first .. last - 1, STEP lanes side by side and four reads under way.
+template <typename I, bool FIRST, int STEP, typename Do>
+__device__ __forceinline__ void sort_walk(const I* ids, const int* keys, int G,
+                                          long first, long last, int lane,
+                                          Do work) {
+  for (long i0 = first; i0 < last; i0 += 4 * STEP) {
+    int key[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const long i = i0 + u * STEP + lane;
+      key[u] = i < last ? sort_key<I, FIRST>(ids, keys, G, (int)i) : 0;
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const long i = i0 + u * STEP + lane;
+      work(i, key[u], i < last);
+    }
+  }
+}
+
 template <typename I, bool FIRST>
 __global__ __launch_bounds__(256) void sort_count_kernel(
     const I* __restrict__ ids, const int* __restrict__ keys, int M, int G,
@@ -146,10 +166,10 @@ __global__ __launch_bounds__(256) void sort_count_kernel(
   __syncthreads();
   const long first = (long)blockIdx.x * tile;
   const int last = (int)min(first + tile, (long)M);
-  for (long i = first + threadIdx.x; i < last; i += 256)
-    atomicAdd(&count[(sort_key<I, FIRST>(ids, keys, G, (int)i) >> shift) &
-                     mask],
-              1);
+  sort_walk<I, FIRST, 256>(ids, keys, G, first, last, threadIdx.x,
+                           [&](long, int key, bool in) {
+                             if (in) atomicAdd(&count[(key >> shift) & mask], 1);
+                           });
   __syncthreads();
   for (int b = threadIdx.x; b < bins; b += 256)
     table[(long)blockIdx.x * bins + b] = count[b];
@@ -252,10 +272,10 @@ __global__ __launch_bounds__(256) void sort_place_kernel(
   const long first = (long)blockIdx.x * tile + (long)wave * part;
   const long last = min(first + part, (long)M);
   int* mine = place + wave * bins;
-  for (long i = first + lane; i < last; i += 64)
-    atomicAdd(&mine[(sort_key<I, FIRST>(ids, keys, G, (int)i) >> shift) &
-                    mask],
-              1);
+  sort_walk<I, FIRST, 64>(ids, keys, G, first, last, lane,
+                          [&](long, int key, bool in) {
+                            if (in) atomicAdd(&mine[(key >> shift) & mask], 1);
+                          });
   __syncthreads();
   for (int b = threadIdx.x; b < bins; b += 256) {
     int at = base[b] + table[(long)blockIdx.x * bins + b];
@@ -268,31 +288,28 @@ __global__ __launch_bounds__(256) void sort_place_kernel(
   }
   __syncthreads();
   volatile int* at = mine;
-  for (long i0 = first; i0 < last; i0 += 64) {
-    const long i = i0 + lane;
-    const bool in = i < last;
-    const int key = in ? sort_key<I, FIRST>(ids, keys, G, (int)i) : 0;
-    const int digit = (key >> shift) & mask;
-    unsigned long long same = __ballot(in);
-    for (int b = 0; b < bits; ++b) {
-      const bool one = (digit >> b) & 1;
-      const unsigned long long set = __ballot(one);
-      same &= one ? set : ~set;
-    }
-    const unsigned long long below = same & ((1ull << lane) - 1);
-    const int rank = __popcll(below);
-    const int start = in ? at[digit] : 0;
-    __builtin_amdgcn_wave_barrier();
-    if (in && rank == 0) at[digit] = start + __popcll(same);
-    __builtin_amdgcn_wave_barrier();
-    if (in) {
-      const int pos = start + rank;
-      const int entry = FIRST ? (int)i : entries[i];
-      order[pos] = entry;
-      if (!LAST || !FIRST) keys_out[pos] = key;
-      if (LAST) slots[entry] = pos;
-    }
-  }
+  sort_walk<I, FIRST, 64>(
+      ids, keys, G, first, last, lane, [&](long i, int key, bool in) {
+        const int digit = (key >> shift) & mask;
+        unsigned long long same = __ballot(in);
+        for (int b = 0; b < bits; ++b) {
+          const bool one = (digit >> b) & 1;
+          const unsigned long long set = __ballot(one);
+          same &= one ? set : ~set;
+        }
+        const int rank = __popcll(same & ((1ull << lane) - 1));
+        const int start = in ? at[digit] : 0;
+        wave_fence();
+        if (in && rank == 0) at[digit] = start + __popcll(same);
+        wave_fence();
+        if (in) {
+          const int pos = start + rank;
+          const int entry = FIRST ? (int)i : entries[i];
+          order[pos] = entry;
+          if (!LAST || !FIRST) keys_out[pos] = key;
+          if (LAST) slots[entry] = pos;
+        }
+      });
 }
 
 __global__ void sort_offsets_kernel(const int* __restrict__ keys, int M,
@@ -320,10 +337,10 @@ void sort_launch(const I* ids, int M, int G, int* offsets, int* slots,
   const int digit = one ? bits : (bits + 1) / 2;
   const int mask = (1 << digit) - 1;
   const int bins = one ? G + 1 : 1 << digit;
-  // 2048 entries a block at least, and not fewer than it has counters; 1024
+  // 2048 entries a block at least, and not fewer than half its counters; 1024
   // blocks at most
   int tile = 2048;
-  while (tile < bins || (long)tile * 1024 < M) tile *= 2;
+  while (tile < bins / 2 || (long)tile * 1024 < M) tile *= 2;
   const int blocks = (int)(((long)M + tile - 1) / tile);
   at::Tensor table = at::empty({(int64_t)bins * blocks + 2 * bins}, opt);
   int* tab = table.data_ptr<int>();
