@@ -80,7 +80,7 @@ def combine_rows_backward_ref(dy, rows, offsets, slots, weights, need_rows,
             spread = spread * weights.to(d.dtype)[..., None]
         drows = torch.empty(T * k, dy.shape[1], dtype=dy.dtype)
         drows[slots.long().reshape(-1)] = spread.reshape(
-            T * k, -1).to(dy.dtype)
+            T * k, dy.shape[1]).to(dy.dtype)
         drows[int(offsets[-1]):] = 0
     if need_weights:
         dot = (_kept(rows, offsets, slots) * d[:, None]).sum(-1)

@@ -582,6 +582,125 @@ def test_plan_of_wild_values_stays_in_bounds():
     assert torch.equal(out[:, 0], x.sum(1))
 
 
+@pytest.mark.gpu
+def test_far_products():
+    """The tile kernels where row addresses pass 32 bits, in both operands
+    and in the gradients; the last rows are compared."""
+    F, N, M = 4096, 72, (1 << 19) + 77
+    gen = torch.Generator().manual_seed(1)
+    rows = torch.zeros(M, F, dtype=torch.bfloat16, device="cuda")
+    rows[M - 90:] = randn(gen, 90, F, dtype=torch.bfloat16, device="cuda")
+    dy = torch.zeros(M, N, dtype=torch.bfloat16, device="cuda")
+    dy[M - 90:] = randn(gen, 90, N, dtype=torch.bfloat16, device="cuda")
+    weight = randn(gen, 2, N, F, dtype=torch.bfloat16, device="cuda")
+    offsets = torch.tensor([0, M - 80, M], dtype=torch.int32, device="cuda")
+    leaves = [rows.requires_grad_(), weight.requires_grad_()]
+    y = ska.grouped_linear(*leaves, offsets)
+    drows, dweight = torch.autograd.grad(y, leaves, dy)
+    r, d = (v[M - 80:].detach().double() for v in (rows, dy))
+    w = weight[1].detach().double()
+    for got, a, b, K in ((y[M - 80:].detach(), r, w.t(), F),
+                         (drows[M - 80:], d, w, N),
+                         (dweight[1], d.t(), r, 80)):
+        check(got, (a @ b).cpu(), (a.abs() @ b.abs()).cpu(), K)
+    assert not y[:M - 90].any() and not drows[:M - 90].any()
+
+
+@pytest.mark.gpu
+def test_far_strides():
+    """Rows of a view that lie further apart than a tile's offsets reach."""
+    gen = torch.Generator().manual_seed(2)
+    wide = torch.zeros(300, 1 << 23, dtype=torch.bfloat16, device="cuda")
+    wide[:, :96] = randn(gen, 300, 96, dtype=torch.bfloat16, device="cuda")
+    rows = wide[:, :96]
+    weight = randn(gen, 2, 80, 96, dtype=torch.bfloat16, device="cuda")
+    offsets = torch.tensor([0, 150, 300], dtype=torch.int32, device="cuda")
+    got = ska.grouped_linear(rows, weight, offsets)
+    assert torch.equal(got, ska.grouped_linear(rows.contiguous(), weight,
+                                               offsets))
+
+
+@pytest.mark.gpu
+def test_two_threads_at_once():
+    """Two threads on streams of their own, as often as each likes."""
+    import threading
+
+    datas = [chain_data("cuda", T=t, G=g, seed=t)
+             for t, g in ((900, 7), (2600, 21))]
+
+    def once(data):
+        x, ids, weight, bias, w, dy = data
+        leaves = [v.detach().requires_grad_() for v in (x, weight, bias, w)]
+        y = chain(leaves[0], ids, weight.shape[0], *leaves[1:])
+        return (y.detach(),) + torch.autograd.grad(y, leaves, dy)
+
+    want = [once(d) for d in datas]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                got = once(datas[i])
+                torch.cuda.current_stream().synchronize()
+                if not all(torch.equal(a, b) for a, b in zip(got, want[i])):
+                    bad.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(60)
+    assert not bad and not any(t.is_alive() for t in threads)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("T,k,F", [(5, 0, 4), (0, 2, 4), (3, 2, 0)])
+def test_moves_of_nothing(device, T, k, F):
+    plan = ska.group_rows(torch.zeros(T, k, dtype=torch.int64,
+                                      device=device), 3)
+    assert plan.offsets.tolist() == [0] + [T * k] * 3
+    x = torch.ones(T, F, device=device, requires_grad=True)
+    w = torch.ones(T, k, device=device, requires_grad=True)
+    y = ska.combine_rows(ska.gather_rows(x, plan), plan, w)
+    assert y.shape == (T, F) and (k or not y.any())
+    dx, dw = torch.autograd.grad(y, [x, w], torch.ones_like(y))
+    assert dx.shape == (T, F) and dw.shape == (T, k) and not dw[:, :0].any()
+    assert F or not dw.any()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("k", [1, 17])
+def test_one_dimension_and_many_entries_a_row(device, k):
+    """ids [T] are ids [T, 1]; a row may go to many groups, to one twice."""
+    gen = torch.Generator().manual_seed(k)
+    T, G, F = 90, 11, 24
+    ids = torch.randint(-1, G, (T, k), generator=gen).to(device)
+    if k == 1:
+        ids = ids[:, 0]
+    x = randn(gen, T, F, device=device).requires_grad_()
+    w = randn(gen, *ids.shape, device=device).requires_grad_()
+    plan = ska.group_rows(ids, G)
+    assert plan.slots.shape == ids.shape
+    y = ska.combine_rows(ska.gather_rows(x, plan), plan, w)
+    kept = (ids >= 0).double()
+    total = (w.detach().double() * kept).reshape(T, -1).sum(1, keepdim=True)
+    size = (w.detach().double().abs() * kept).reshape(T, -1).sum(
+        1, keepdim=True)
+    xd = x.detach().double()
+    check(y.detach(), (xd * total).cpu(), (xd.abs() * size).cpu(), k + 1)
+    dy = randn(gen, T, F, device=device)
+    dx, dw = torch.autograd.grad(y, [x, w], dy)
+    assert dw.shape == w.shape
+    dots = (xd * dy.double()).sum(1, keepdim=True)
+    mags = (xd * dy.double()).abs().sum(1, keepdim=True)
+    shape = (T, -1)
+    check(dw.reshape(shape), (dots * kept.reshape(shape)).cpu(),
+          (mags * kept.reshape(shape)).cpu(), F)
+    check(dx, (dy.double() * total).cpu(),
+          (dy.double().abs() * size).cpu(), k + 1)
+
+
 # -- refusals -----------------------------------------------------------------
 
 def small():
