@@ -1935,8 +1935,8 @@ void product_launch(Product p, at::TensorOptions opt) {
   //            60000, 300,  720,  40:   60 /  45 /   42 /   31
   //
   // One tile of c at a time, where enough blocks share a CU (us with two / one
-  // at 128^2): forward 28273, 179, 2072, 84: 93 / 71; 40000, 400, 512, 512:
-  // 64 / 60; but drows 3000, 64, 64, 1024: 16 / 20.
+  // at 128^2): forward 28273, 179, 2072, 84: 93 / 71; 8192, 8, 1024, 1024:
+  // 37 / 32; but 2048, 16, 2048, 2048: 40 / 48.
   constexpr bool kWide = sizeof(T) == 4;  // float32 has no larger ones
   constexpr long KS = 128 / sizeof(T);
   auto tile128 = [&](bool ahead) {
@@ -1957,22 +1957,21 @@ void product_launch(Product p, at::TensorOptions opt) {
   };
   const long each =  // rows a group
       MODE == kDWeight ? p.C / p.G : p.M / std::min(p.G, p.M);
-  auto ahead = [&](long blocks) {
-    return blocks < 1024 && (MODE == kDWeight ? each : p.C) > 2 * KS;
+  auto ahead = [&](long blocks, long enough) {
+    return blocks < enough && (MODE == kDWeight ? each : p.C) > 2 * KS;
   };
   if (MODE == kDWeight) {
-    // 256^2 where that fills the card twice and its edges waste less than a
-    // third
-    const bool large = p.G * tiles(256) >= 512 &&
+    // 256^2 where that fills the card and its edges waste less than a third
+    const bool large = p.G * tiles(256) >= 400 &&
                        tiles(256) * 65536 * 3 <= 4l * p.M * p.N;
     const bool middle = p.M > 64 && p.N > 64 && p.G * tiles(128) >= 256;
     if (large && async && !kWide) {
       if constexpr (!kWide)
         go(product_kernel<T, 256, 256, 2, 4, MODE, true>, 256, 256, 512);
     } else if (large || middle) {
-      tile128(ahead(p.G * tiles(128)));
+      tile128(ahead(p.G * tiles(128), 512));
     } else {
-      tile64(ahead(p.G * tiles(64)));
+      tile64(ahead(p.G * tiles(64), 1024));
     }
     return;
   }
@@ -1987,14 +1986,14 @@ void product_launch(Product p, at::TensorOptions opt) {
     if constexpr (!kWide)
       go(product_kernel<T, 256, 256, 2, 4, MODE, true>, 256, 256, 512);
   } else if (large || middle) {
-    tile128(ahead(row_tiles(128, 128)));
+    tile128(ahead(row_tiles(128, 128), 512));
   } else if (async && p.N > 64 && row_tiles(64, 128) >= 256) {
-    if (ahead(row_tiles(64, 128)))
+    if (ahead(row_tiles(64, 128), 768))
       go(product_kernel<T, 64, 128, 1, 4, MODE, true>, 64, 128, 256);
     else
       go(product_kernel<T, 64, 128, 1, 4, MODE, true, false>, 64, 128, 256);
   } else {
-    tile64(ahead(row_tiles(64, 64)));
+    tile64(ahead(row_tiles(64, 64), 1024));
   }
 }
 
