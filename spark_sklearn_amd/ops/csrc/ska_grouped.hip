@@ -1306,7 +1306,7 @@ __device__ __forceinline__ bool find_job(const Product& p, int tile,
 // each other's loads and of which more then fit a CU.
 template <typename T, int BM, int BN, int WM, int WN, int MODE, bool ASYNC,
           bool AHEAD = true>
-__global__ __launch_bounds__(WM* WN * 64) void product_kernel(Product p) {
+__global__ __launch_bounds__(WM* WN * 64, 2) void product_kernel(Product p) {
   constexpr int kThreads = WM * WN * 64;
   constexpr int FM = BM / WM / 16, FN = BN / WN / 16;
   typedef Tile<T, BM, MODE == kDWeight, kThreads, 1> TA;
@@ -1359,10 +1359,17 @@ __global__ __launch_bounds__(WM* WN * 64) void product_kernel(Product p) {
     TB::load_regs(s.b, p.b_pitch, job.cols, s.steps, s.bb, rb);
   };
   f32x4 acc[FM][FN] = {};
+  // The sums of the weights' gradients go over a group's rows, as many as these
+  // may be.  In float32 they are taken in parts of 512 rows, since an addition's
+  // rounding grows with the sum so far: over 32768 rows they are 4e-7 off (in
+  // the 2-norm), a library's single sum 3e-6.  16-bit results round far more.
+  constexpr bool PARTS = sizeof(T) == 4 && MODE == kDWeight;
+  constexpr int kPart = 512 / KS;
+  f32x4 total[PARTS ? FM : 1][PARTS ? FN : 1] = {};
   // The sums over c of A: a product with ones, of which each of the WN waves
   // that hold the same rows takes FS fragments.
   constexpr int FS = FM / WN > 0 ? FM / WN : 1;
-  f32x4 sum[FS] = {};
+  f32x4 sum[FS] = {}, total_sum[FS] = {};
   const bool sums = MODE == kDWeight && p.sums && job.n0 == 0;
   const int mine = wave % WN;
   typename Mma<T>::Frag ones;
@@ -1431,6 +1438,22 @@ __global__ __launch_bounds__(WM* WN * 64) void product_kernel(Product p) {
       if (MODE == kDWeight && sums && i / FS == mine)
         sum[i % FS] = Mma<T>::go(ones, fa[g & 1], sum[i % FS]);
       __builtin_amdgcn_sched_barrier(0);
+    }
+    if constexpr (PARTS) {
+      if (c / KS % kPart == kPart - 1 || next.steps <= 0) {
+#pragma unroll
+        for (int i = 0; i < FM; ++i)
+#pragma unroll
+          for (int j = 0; j < FN; ++j) {
+            total[i][j] += acc[i][j];
+            acc[i][j] = next.steps > 0 ? f32x4{} : total[i][j];
+          }
+#pragma unroll
+        for (int i = 0; i < FS; ++i) {
+          total_sum[i] += sum[i];
+          sum[i] = next.steps > 0 ? f32x4{} : total_sum[i];
+        }
+      }
     }
     if constexpr (AHEAD) {
       buf ^= 1;
@@ -1958,9 +1981,10 @@ void product_launch(Product p, at::TensorOptions opt) {
   const long each =  // rows a group
       MODE == kDWeight ? p.C / p.G : p.M / std::min(p.G, p.M);
   auto ahead = [&](long blocks, long enough) {
-    return blocks < enough && (MODE == kDWeight ? each : p.C) > 2 * KS;
+    // (the float32 instructions take eight times as long: always worth it)
+    return (kWide || blocks < enough) && (MODE == kDWeight ? each : p.C) > 2 * KS;
   };
-  if (MODE == kDWeight) {
+  if constexpr (MODE == kDWeight) {
     // 256^2 where that fills the card and its edges waste less than a third
     const bool large = p.G * tiles(256) >= 400 &&
                        tiles(256) * 65536 * 3 <= 4l * p.M * p.N;
@@ -1973,27 +1997,27 @@ void product_launch(Product p, at::TensorOptions opt) {
     } else {
       tile64(ahead(p.G * tiles(64), 1024));
     }
-    return;
-  }
-  auto row_tiles = [&](long bm, long bn) {
-    return (p.M / bm + std::min(p.G, p.M) / 2 + 1) * ((p.N + bn - 1) / bn);
-  };
-  const bool large = each >= 768 && p.N > 128 && row_tiles(256, 256) >= 512;
-  const bool middle =
-      p.N > 64 && ((each >= 192 && row_tiles(128, 128) >= 256) ||
-                   (each >= 96 && row_tiles(128, 128) >= 1024));
-  if (large && async && !kWide) {
-    if constexpr (!kWide)
-      go(product_kernel<T, 256, 256, 2, 4, MODE, true>, 256, 256, 512);
-  } else if (large || middle) {
-    tile128(ahead(row_tiles(128, 128), 512));
-  } else if (async && p.N > 64 && row_tiles(64, 128) >= 256) {
-    if (ahead(row_tiles(64, 128), 768))
-      go(product_kernel<T, 64, 128, 1, 4, MODE, true>, 64, 128, 256);
-    else
-      go(product_kernel<T, 64, 128, 1, 4, MODE, true, false>, 64, 128, 256);
   } else {
-    tile64(ahead(row_tiles(64, 64), 1024));
+    auto row_tiles = [&](long bm, long bn) {
+      return (p.M / bm + std::min(p.G, p.M) / 2 + 1) * ((p.N + bn - 1) / bn);
+    };
+    const bool large = each >= 768 && p.N > 128 && row_tiles(256, 256) >= 512;
+    const bool middle =
+        p.N > 64 && ((each >= 192 && row_tiles(128, 128) >= 256) ||
+                     (each >= 96 && row_tiles(128, 128) >= 1024));
+    if (large && async && !kWide) {
+      if constexpr (!kWide)
+        go(product_kernel<T, 256, 256, 2, 4, MODE, true>, 256, 256, 512);
+    } else if (large || middle) {
+      tile128(ahead(row_tiles(128, 128), 512));
+    } else if (async && p.N > 64 && row_tiles(64, 128) >= 256) {
+      if (ahead(row_tiles(64, 128), 768))
+        go(product_kernel<T, 64, 128, 1, 4, MODE, true>, 64, 128, 256);
+      else
+        go(product_kernel<T, 64, 128, 1, 4, MODE, true, false>, 64, 128, 256);
+    } else {
+      tile64(ahead(row_tiles(64, 64), 1024));
+    }
   }
 }
 

@@ -340,6 +340,28 @@ def test_grouped_linear_keeps_groups_apart(device, dtype):
         assert torch.equal(a, b)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,G,N,F", [(8192, 1, 2048, 2048),
+                                     (30000, 2, 70, 100), (30000, 1, 9, 64)])
+def test_long_sums_in_parts(M, G, N, F):
+    """float32 weight gradients sum at most 512 terms, and then those sums:
+    a term passes 512 + M / 512 + 1 additions."""
+    gen = torch.Generator().manual_seed(M)
+    offsets = offsets_of("even", M, G)
+    rows, grad = (randn(gen, M, v, device="cuda") for v in (F, N))
+    weight = torch.zeros(G, N, F, device="cuda", requires_grad=True)
+    bias = torch.zeros(G, N, device="cuda", requires_grad=True)
+    y = ska.grouped_linear(rows, weight, offsets.cuda(), bias)
+    dweight, dbias = torch.autograd.grad(y, [weight, bias], grad)
+    r, d = rows.double(), grad.double()
+    edges = offsets.tolist()
+    for g, (a, b) in enumerate(zip(edges, edges[1:])):
+        check(dweight[g], (d[a:b].t() @ r[a:b]).cpu(),
+              (d[a:b].t().abs() @ r[a:b].abs()).cpu(), 513 + M // 512)
+        check(dbias[g], d[a:b].sum(0).cpu(), d[a:b].abs().sum(0).cpu(),
+              513 + M // 512)
+
+
 @pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("M,G,N,F", [(0, 3, 4, 5), (7, 3, 0, 5),
                                      (7, 3, 4, 0), (0, 1, 0, 0)])
