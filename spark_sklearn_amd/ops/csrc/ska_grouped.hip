@@ -82,8 +82,8 @@ __device__ __forceinline__ void wave_fence() {
 
 // Few entries: one block sorts key * 2048 + entry, which makes the order
 // stable, in LDS: compare and exchange at distances of halves.  Distances
-// below 64 stay within a wave, where no barrier is needed.  2012 entries took
-// 158 us by comparing each with every other.
+// up to 64 stay within a wave, where no barrier is needed.  (Comparing each of
+// 2012 entries with every other took 158 us.)
 template <typename I>
 __global__ __launch_bounds__(1024) void sort_small_kernel(
     const I* __restrict__ ids, int M, int G, int size,
@@ -323,10 +323,15 @@ template <typename I>
 void sort_launch(const I* ids, int M, int G, int* offsets, int* slots,
                  int* order, at::TensorOptions opt) {
   hipStream_t s = stream_now();
-  if (M <= kSmallEntries && G <= kSmallGroups) {
+  // us for 100 / 1000 / 2048 entries in one block, and in the passes below:
+  // 64 groups 7 / 14 / 20, and 13; 4096 groups 9 / 16 / 23, and 28
+  if (M <= (G < 2048 ? kSmallEntries / 2 : kSmallEntries) &&
+      G <= kSmallGroups) {
     int size = 2;
     while (size < M) size *= 2;
-    sort_small_kernel<I><<<1, std::min(1024, std::max(64, size / 2)), 0, s>>>(
+    // size / 2 threads sort, G + 1 look up offsets
+    const int threads = std::max(size / 2, std::min(1024, G + 1));
+    sort_small_kernel<I><<<1, (threads + 63) / 64 * 64, 0, s>>>(
         ids, M, G, size, offsets, slots, order);
     check_launch();
     return;
@@ -337,10 +342,14 @@ void sort_launch(const I* ids, int M, int G, int* offsets, int* slots,
   const int digit = one ? bits : (bits + 1) / 2;
   const int mask = (1 << digit) - 1;
   const int bins = one ? G + 1 : 1 << digit;
-  // 2048 entries a block at least, and not fewer than half its counters; 1024
-  // blocks at most
-  int tile = 2048;
-  while (tile < bins / 2 || (long)tile * 1024 < M) tile *= 2;
+  // 512 entries a block at least, and not fewer than half its counters; about
+  // 256 blocks while these are short, and as many at most as the scan of their
+  // counts is worth
+  const long most = bins <= 1024 ? 4096 : 1024;
+  int tile = 512;
+  while (tile < bins / 2 || (tile * 256l < M && tile < 8192) ||
+         tile * most < M)
+    tile *= 2;
   const int blocks = (int)(((long)M + tile - 1) / tile);
   at::Tensor table = at::empty({(int64_t)bins * blocks + 2 * bins}, opt);
   int* tab = table.data_ptr<int>();
