@@ -108,7 +108,7 @@ __global__ __launch_bounds__(1024) void sort_small_kernel(
           item[b] = x;
         }
       }
-      // 64 threads own 128 neighbouring elements while d < 64
+      // a wave's 64 threads own 128 neighbouring elements while d <= 64
       if (d > 64 || (d == 1 && run >= 64))
         __syncthreads();
       else
@@ -127,6 +127,10 @@ __global__ __launch_bounds__(1024) void sort_small_kernel(
 // Many entries: passes over a digit of the key, low digit first.  One pass
 // sorts up to kBins keys; more groups take two.  A pass counts each block's
 // digits, sums the counts over the blocks before it, and places the entries.
+// No atomic decides an order, so that the sort is stable.  10^6 entries take
+// 32 us for 64 groups and 56 for 4096 (10 and 23 us of it counting and
+// placing); what bounds it is the chain of LDS accesses of 64 entries after
+// the other, and 4-byte stores to places apart.
 constexpr int kBins = 8192;
 constexpr int kSortWaves = 4;
 
@@ -168,7 +172,8 @@ __global__ __launch_bounds__(256) void sort_count_kernel(
   const int last = (int)min(first + tile, (long)M);
   sort_walk<I, FIRST, 256>(ids, keys, G, first, last, threadIdx.x,
                            [&](long, int key, bool in) {
-                             if (in) atomicAdd(&count[(key >> shift) & mask], 1);
+                             const int digit = (key >> shift) & mask;
+                             if (in) atomicAdd(&count[digit], 1);
                            });
   __syncthreads();
   for (int b = threadIdx.x; b < bins; b += 256)
@@ -274,7 +279,8 @@ __global__ __launch_bounds__(256) void sort_place_kernel(
   int* mine = place + wave * bins;
   sort_walk<I, FIRST, 64>(ids, keys, G, first, last, lane,
                           [&](long, int key, bool in) {
-                            if (in) atomicAdd(&mine[(key >> shift) & mask], 1);
+                            const int digit = (key >> shift) & mask;
+                            if (in) atomicAdd(&mine[digit], 1);
                           });
   __syncthreads();
   for (int b = threadIdx.x; b < bins; b += 256) {
@@ -500,6 +506,10 @@ __device__ __forceinline__ void put(T* p, const Vec<T>& r) {
   *reinterpret_cast<Bytes16*>(p) = __builtin_bit_cast(Bytes16, r.v);
 }
 
+// In row order, so that a row is read once for its k places.  Bound by memory:
+// 10^6 rows of 256 float32 move in 365 us (5.6 TB/s, where a copy of that size
+// has 5.4).  Loads that the compiler took apart into pieces of 2 bytes, because
+// the values' type was an array, had 3.1.
 template <typename T, int U>
 __global__ __launch_bounds__(256) void gather_kernel(
     const T* __restrict__ x, long x_pitch, const int* __restrict__ slots,
@@ -608,7 +618,8 @@ __global__ __launch_bounds__(256) void combine_kernel(
 }
 
 // Backward of combine, in row order: dy[t] is read once for J rows, each row
-// once; drows (where asked for) and the dot products leave with them.
+// once; drows (where asked for) and the dot products leave with them.  Bound by
+// memory: 8191 x 2 rows of 1001 float16 take 20 us (4.1 TB/s).
 template <typename T, typename W, int J, int U>
 __global__ __launch_bounds__(256) void combine_back_kernel(
     const T* __restrict__ dy, long dy_pitch, const T* __restrict__ rows,
@@ -1062,7 +1073,7 @@ struct Tile {
     if (FRAGS == 1)
       return (((c & 3) << 1) | (((c >> 3) & 1) << 3)) & (kAcross - 1);
     if (FRAGS == 2)
-      return ((c & 1) | ((c & 2) << 1) | ((c & 8) >> 0)) & (kAcross - 1);
+      return ((c & 1) | ((c & 2) << 1) | (c & 8)) & (kAcross - 1);
     return ((c & 1) | ((c & 2) << 2)) & (kAcross - 1);
   }
   // the first row and step of the granule at LDS place g
@@ -1310,6 +1321,16 @@ __device__ __forceinline__ bool find_job(const Product& p, int tile,
   return true;
 }
 
+// 8192^3 bfloat16 in one group: 858 us, 1281 TFLOP/s (1308 for a library's
+// product); 65536 x 2048 x 1024 in 64 groups: 319 us, 862, since the groups'
+// last tiles are half empty and 1160 tiles take five rounds of 256 CUs, not
+// 4.5. What it took from there on: loads spread among the matrix instructions
+// (1166 -> 1067 us at 8192^3; all at once they hold up the waves) and the
+// bands of find_job (-> 895: half of the L2 reads had missed).  What did not
+// help: four waves with fragments of two half steps (797 TFLOP/s), waves that
+// take turns at LDS and the matrix unit (708), three tiles in LDS, one block a
+// CU that goes through many tiles.
+//
 // Tiles of c in LDS, filled by loads that write it (ASYNC) or through
 // registers: two, or one (not AHEAD) for short contractions, whose blocks hide
 // each other's loads and of which more then fit a CU.
@@ -1368,10 +1389,11 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void product_kernel(Product p) {
     TB::load_regs(s.b, p.b_pitch, job.cols, s.steps, s.bb, rb);
   };
   f32x4 acc[FM][FN] = {};
-  // The sums of the weights' gradients go over a group's rows, as many as these
-  // may be.  In float32 they are taken in parts of 512 rows, since an addition's
-  // rounding grows with the sum so far: over 32768 rows they are 4e-7 off (in
-  // the 2-norm), a library's single sum 3e-6.  16-bit results round far more.
+  // The sums of the weights' gradients go over a group's rows, as many as
+  // these may be.  In float32 they are taken in parts of 512 rows, since an
+  // addition's rounding grows with the sum so far: over 32768 rows they are
+  // 4e-7 off (in the 2-norm), a library's single sum 3e-6.  16-bit results
+  // round far more.
   constexpr bool PARTS = sizeof(T) == 4 && MODE == kDWeight;
   constexpr int kPart = 512 / KS;
   f32x4 total[PARTS ? FM : 1][PARTS ? FN : 1] = {};
@@ -1565,12 +1587,14 @@ __global__ __launch_bounds__(256) void finish_kernel(Product p) {
 }
 
 // ---------------------------------------------------------------------------
-// Narrow forward products: few outputs (a keyed model's classes) or few rows
-// a group (single rows of a serving step).  The larger operand is read once,
-// straight from memory into fragments: a lane takes 16 bytes of row lane & 15
-// at the contraction's step (lane >> 4) * V, and both operands agree on which
-// steps these are, so their order in the instruction does not matter.
-// KW of the 4 waves share the contraction, the others lie along the rows.
+// Narrow forward products: few outputs (a keyed model's classes) or few rows a
+// group (single rows of a serving step).  Bound by reading the larger operand,
+// once: 8 rows x 2048 x 2048 bfloat16 in 12.4 us (5.4 TB/s), 10^6 x 256
+// float32 with 10 outputs in 218 us (4.9).  It goes straight from memory into
+// fragments: a lane takes 16 bytes of row lane & 15 at the contraction's step
+// (lane >> 4) * V, and both operands agree on which steps these are, so their
+// order in the instruction does not matter. KW of the 4 waves share the
+// contraction, the others lie along the rows.
 // ---------------------------------------------------------------------------
 template <typename T>
 struct Wide {
@@ -1698,11 +1722,11 @@ __global__ __launch_bounds__(256) void narrow_kernel(Product p, bool by_row) {
   }
 }
 
-// float32 dweight with few outputs: dw[g, n, f] for 16 outputs.  A lane takes 4
-// columns f = 4 * (lane & 15) + e of the row (lane >> 4) * 4 + i, which are four
-// fragments' values at once.  KW of the 4 waves share the rows, the others lie
-// along f.  Bound by reading the rows: 400000 x 256 with 3 outputs in 512
-// groups take 86 us (4.8 TB/s; 64^2 tiles 171).
+// float32 dweight with few outputs: dw[g, n, f] for 16 outputs.  A lane takes
+// 4 columns f = 4 * (lane & 15) + e of the row (lane >> 4) * 4 + i, which are
+// four fragments' values at once.  KW of the 4 waves share the rows, the
+// others lie along f.  Bound by reading the rows: 400000 x 256 with 3 outputs
+// in 512 groups take 86 us (4.8 TB/s; 64^2 tiles 171).
 template <int KW>
 __global__ __launch_bounds__(256) void narrow_dweight_kernel(Product p) {
   constexpr int BF = 4 / KW * 64;
@@ -1846,7 +1870,7 @@ bool whole_words(const T* p, long pitch) {
 }
 
 unsigned grid_of(long blocks, int threads) {
-  TORCH_CHECK(blocks * threads < (1ll << 32), "too many tiles");
+  TORCH_CHECK(blocks * threads < (1ll << 32), "too many output tiles");
   return (unsigned)blocks;
 }
 
@@ -1945,7 +1969,7 @@ void product_launch(Product p, at::TensorOptions opt) {
       }
     }
     mt *= p.out ? (p.N + bn - 1) / bn : 1;
-    TORCH_CHECK(mt * threads < (1ll << 31), "too many tiles");
+    grid_of(mt + 7, threads);
     p.tiles = (int)mt;
     kern<<<(unsigned)((mt + 7) / 8 * 8), threads, 0, stream_now()>>>(p);
     check_launch();
@@ -1991,7 +2015,8 @@ void product_launch(Product p, at::TensorOptions opt) {
       MODE == kDWeight ? p.C / p.G : p.M / std::min(p.G, p.M);
   auto ahead = [&](long blocks, long enough) {
     // (the float32 instructions take eight times as long: always worth it)
-    return (kWide || blocks < enough) && (MODE == kDWeight ? each : p.C) > 2 * KS;
+    return (kWide || blocks < enough) &&
+           (MODE == kDWeight ? each : p.C) > 2 * KS;
   };
   if constexpr (MODE == kDWeight) {
     // 256^2 where that fills the card and its edges waste less than a third
