@@ -1240,6 +1240,7 @@ struct Product {
   float* part;
   float* part_sums;
   int tiles;  // output tiles of the launch
+  int run;    // of neighbouring tiles that go to one XCD
 };
 
 // One tile of the output: its operands and where it goes.
@@ -1345,10 +1346,11 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void product_kernel(Product p) {
   static_assert(ASYNC || AHEAD);
   __shared__ __align__(16) char lds[AHEAD ? 2 : 1][TA::kBytes + TB::kBytes];
 
-  // Blocks go round the 8 XCDs: each XCD gets a contiguous run of tiles, whose
+  // Blocks go round the 8 XCDs: each XCD gets runs of neighbouring tiles, whose
   // operands its L2 then holds.
-  const int run = (p.tiles + 7) >> 3;
-  const int tile = (blockIdx.x & 7) * run + (blockIdx.x >> 3);
+  const int at = blockIdx.x >> 3;
+  const int tile =
+      (at / p.run * 8 + (blockIdx.x & 7)) * p.run + at % p.run;
   Job<T> job;
   if (tile >= p.tiles || !find_job<T, BM, BN, MODE>(p, tile, job)) return;
 
@@ -1968,10 +1970,22 @@ void product_launch(Product p, at::TensorOptions opt) {
         mt = ((p.C >> p.shift) + p.G + 1) * m_tiles;
       }
     }
-    mt *= p.out ? (p.N + bn - 1) / bn : 1;
-    grid_of(mt + 7, threads);
-    p.tiles = (int)mt;
-    kern<<<(unsigned)((mt + 7) / 8 * 8), threads, 0, stream_now()>>>(p);
+    const long nt = p.out ? (p.N + bn - 1) / bn : 1;
+    grid_of(mt * nt + 512, threads);
+    p.tiles = (int)(mt * nt);
+    // One run an XCD shares most; shorter ones spread large groups.  us for
+    // one run / 16 tiles: forward 65536, 64, 1024, 2048: 345 / 305, but 65536,
+    // 32, 4096, 1024: 593 / 634; dweight of the latter 696 / 598, and with more
+    // skewed groups 894 / 653, but 8198, 48, 768, 768 (9 tiles a group): 32 / 39
+    const long each = m_tiles * nt;
+    long most = p.tiles;
+    if (MODE == kDWeight)
+      most = each > 16 ? 16 : each * std::max(1l, 8 / each);
+    else if (bm == 256 && nt <= 4)
+      most = 16;
+    p.run = (int)std::min(most, (p.tiles + 7l) / 8);
+    const long round = 8 * p.run;
+    kern<<<(unsigned)((p.tiles + round - 1) / round * round), threads, 0, stream_now()>>>(p);
     check_launch();
     if (MODE == kDWeight && p.shift) finish_launch<T>(p);
   };
@@ -2104,7 +2118,7 @@ at::Tensor product(const at::Tensor& a_in, const at::Tensor& weight,
   Product p{a.data_ptr(), weight.data_ptr(),
             bias ? bias->data_ptr() : nullptr, out.data_ptr(), nullptr,
             offsets.data_ptr<int>(), a.stride(0), transposed ? N : C, G, M, N,
-            C, 0, nullptr, nullptr, 0};
+            C, 0, nullptr, nullptr, 0, 0};
   SKA_TYPES(a.scalar_type(), [&] {
     if (transposed && C <= 16)
       narrow_drows_launch<T>(p);
@@ -2153,7 +2167,7 @@ grouped_linear_dweight(const at::Tensor& dy_in, const at::Tensor& rows_in,
   Product p{dy.data_ptr(), b.data_ptr(), nullptr,
             F && dw ? dw->data_ptr() : nullptr, db ? db->data_ptr() : nullptr,
             offsets.data_ptr<int>(), dy.stride(0), b.stride(0), G, N,
-            F ? F : N, M, 0, nullptr, nullptr, 0};
+            F ? F : N, M, 0, nullptr, nullptr, 0, 0};
   SKA_TYPES(dy.scalar_type(), [&] {
     if (sizeof(T) == 4 && N <= 16)
       narrow_dweight_launch(p, dy.options());
