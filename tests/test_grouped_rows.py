@@ -306,6 +306,50 @@ def test_grouped_linear(device, dtype, apart, M, G, N, F, case):
         check(v, u, s, K)
 
 
+def check_there(got, want, scale, K):
+    """check(), where the operands are."""
+    info = torch.finfo(got.dtype)
+    tol = (info.eps / 2 * want.abs() + (K + 1) * 2.0 ** -23 * scale
+           + info.tiny * info.eps) * (1 + info.eps)
+    off = (got.double() - want).abs() - tol
+    assert bool((off <= 0).all()), float(off.max())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=SHORT.get)
+@pytest.mark.parametrize("M,G,N,F", [
+    (24000, 20, 1200, 1250),    # the largest tiles, in all three products
+    (24000, 20, 1200, 1251),    # the same with rows at odd addresses
+    (6000, 16, 700, 300),       # middle tiles, two steps in LDS
+    (20000, 60, 520, 200),      # and one
+    (9000, 100, 520, 140),      # low tiles, one step
+    (6000, 90, 520, 700),       # and two
+    (5000, 3, 37, 600),         # few outputs
+])
+def test_grouped_linear_tiles(dtype, M, G, N, F):
+    """Sizes at which each of the tiles is taken, ragged everywhere."""
+    gen = torch.Generator().manual_seed(N)
+    offsets = offsets_of("ragged", M, G, seed=F)
+    offsets[-1] -= 3            # rows behind the last group
+    rows, weight, bias, grad = (
+        randn(gen, *shape, dtype=dtype, device="cuda")
+        for shape in ((M, F), (G, N, F), (G, N), (M, N)))
+    leaves = [v.requires_grad_() for v in (rows, weight, bias)]
+    y = ska.grouped_linear(rows, weight, offsets.cuda(), bias)
+    dr, dw, db = torch.autograd.grad(y, leaves, grad)
+    y = y.detach()
+    edges = offsets.tolist()
+    for g, (a, b) in enumerate(zip(edges, edges[1:])):
+        r, w, c, d = (v.detach().double() for v in (
+            rows[a:b], weight[g], bias[g], grad[a:b]))
+        R, W, C, D = (v.abs() for v in (r, w, c, d))
+        check_there(y[a:b], r @ w.t() + c, R @ W.t() + C, F + 1)
+        check_there(dr[a:b], d @ w, D @ W, N)
+        check_there(dw[g], d.t() @ r, D.t() @ R, M)
+        check_there(db[g], d.sum(0), D.sum(0), M)
+    assert not y[M - 3:].any() and not dr[M - 3:].any()
+
+
 @pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("dtype", TYPES, ids=SHORT.get)
 def test_grouped_linear_keeps_groups_apart(device, dtype):
@@ -793,6 +837,64 @@ def test_grouped_linear_refuses():
             (dict(bias=1.0), TypeError)]:
         with pytest.raises(error):
             ska.grouped_linear(**{**ok, **change})
+
+
+@pytest.mark.gpu
+def test_refuses_the_same_on_the_gpu():
+    """The kernels' checks raise what the reference's raise."""
+    ids, plan, x, rows, weight = small()
+    w = torch.ones(3, 2)
+    calls = [
+        lambda c: ska.group_rows(c(ids).float(), 3),
+        lambda c: ska.group_rows(c(ids).short(), 3),
+        lambda c: ska.group_rows(c(ids), 0),
+        lambda c: ska.group_rows(c(ids), 1 << 24),
+        lambda c: ska.group_rows(c(ids), 1 << 70),
+        lambda c: ska.group_rows(c(ids), 2.0),
+        lambda c: ska.group_rows(c(ids)[None], 3),
+        lambda c: ska.gather_rows(c(x).int(), p(c)),
+        lambda c: ska.gather_rows(c(x)[0], p(c)),
+        lambda c: ska.gather_rows(c(x)[:2], p(c)),
+        lambda c: ska.gather_rows(c(x), tuple(p(c))),
+        lambda c: ska.gather_rows(c(x), None),
+        lambda c: ska.gather_rows(c(x), p(c)._replace(
+            slots=p(c).slots.long())),
+        lambda c: ska.gather_rows(c(x), p(c)._replace(
+            offsets=p(c).offsets[:1])),
+        lambda c: ska.gather_rows(c(x), p(c)._replace(offsets=3)),
+        lambda c: ska.combine_rows(c(rows)[:5], p(c)),
+        lambda c: ska.combine_rows(c(rows), p(c), c(w)[:2]),
+        lambda c: ska.combine_rows(c(rows), p(c), c(w).half()),
+        lambda c: ska.combine_rows(c(rows), p(c), c(w)[:, 0]),
+        lambda c: ska.combine_rows(c(rows), p(c), [[1.0]]),
+        lambda c: ska.combine_rows(c(rows), None),
+        lambda c: ska.grouped_linear(c(rows)[:, :3], c(weight),
+                                     p(c).offsets),
+        lambda c: ska.grouped_linear(c(rows).bfloat16(), c(weight),
+                                     p(c).offsets),
+        lambda c: ska.grouped_linear(c(rows), c(weight)[0], p(c).offsets),
+        lambda c: ska.grouped_linear(c(rows), c(weight)[:0], p(c).offsets),
+        lambda c: ska.grouped_linear(c(rows), c(weight), p(c).offsets[:3]),
+        lambda c: ska.grouped_linear(c(rows), c(weight),
+                                     p(c).offsets.long()),
+        lambda c: ska.grouped_linear(c(rows), c(weight), p(c).offsets,
+                                     torch.ones(3)),
+        lambda c: ska.grouped_linear(c(rows), c(weight), p(c).offsets,
+                                     c(torch.ones(3, 2)).half()),
+        lambda c: ska.grouped_linear(c(rows), weight.numpy(), p(c).offsets),
+        lambda c: ska.grouped_linear(c(rows), c(weight), p(c).offsets, 1.0),
+    ]
+
+    def p(c):
+        return ska.GroupPlan(*(c(v) for v in plan))
+
+    for i, call in enumerate(calls):
+        raised = []
+        for c in (lambda v: v, lambda v: v.cuda()):
+            with pytest.raises((TypeError, ValueError)) as info:
+                call(c)
+            raised.append(info.type)
+        assert raised[0] is raised[1], (i, raised)
 
 
 @pytest.mark.gpu
