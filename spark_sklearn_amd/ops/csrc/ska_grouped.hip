@@ -1323,7 +1323,7 @@ __device__ __forceinline__ bool find_job(const Product& p, int tile,
 }
 
 // 8192^3 bfloat16 in one group: 858 us, 1281 TFLOP/s (1308 for a library's
-// product); 65536 x 2048 x 1024 in 64 groups: 319 us, 862, since the groups'
+// product); 65536 x 2048 x 1024 in 64 groups: 310 us, 886, since the groups'
 // last tiles are half empty and 1160 tiles take five rounds of 256 CUs, not
 // 4.5. What it took from there on: loads spread among the matrix instructions
 // (1166 -> 1067 us at 8192^3; all at once they hold up the waves) and the
@@ -1883,7 +1883,7 @@ bool narrow_launch(const Product& p) {
     const bool by_row = p.M < p.M / bm + p.G + 1;
     const long tiles = by_row ? p.M : p.M / bm + p.G + 1;
     dim3 grid(grid_of(tiles, 256), (p.N + bn - 1) / bn);
-    TORCH_CHECK(grid.y < 65536, "rows are too wide");
+    if (grid.y > 65535) return false;  // more than a launch takes
     kern<<<grid, 256, 0, stream_now()>>>(p, by_row);
     check_launch();
     return true;
@@ -1985,7 +1985,8 @@ void product_launch(Product p, at::TensorOptions opt) {
       most = 16;
     p.run = (int)std::min(most, (p.tiles + 7l) / 8);
     const long round = 8 * p.run;
-    kern<<<(unsigned)((p.tiles + round - 1) / round * round), threads, 0, stream_now()>>>(p);
+    const unsigned blocks = (unsigned)((p.tiles + round - 1) / round * round);
+    kern<<<blocks, threads, 0, stream_now()>>>(p);
     check_launch();
     if (MODE == kDWeight && p.shift) finish_launch<T>(p);
   };
@@ -2075,7 +2076,6 @@ void narrow_dweight_launch(Product p, at::TensorOptions opt) {
   p.shift = part_shift(p.C, tiles, 2048);
   Parts parts = take_parts(p, opt);
   dim3 grid(grid_of(((long)p.C >> p.shift) + p.G + 1, 256), p.out ? tiles : 1);
-  TORCH_CHECK(grid.y < 65536, "rows are too wide");
   if (kw == 4)
     narrow_dweight_kernel<4><<<grid, 256, 0, stream_now()>>>(p);
   else

@@ -350,6 +350,28 @@ def test_grouped_linear_tiles(dtype, M, G, N, F):
     assert not y[M - 3:].any() and not dr[M - 3:].any()
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=SHORT.get)
+def test_grouped_linear_most_outputs(dtype):
+    """As many outputs as there may be, for a few rows."""
+    M, N, F = 3, 2 ** 21 - 1, 4
+    gen = torch.Generator().manual_seed(5)
+    rows, weight, bias, grad = (
+        randn(gen, *shape, dtype=dtype, device="cuda")
+        for shape in ((M, F), (1, N, F), (1, N), (M, N)))
+    offsets = torch.tensor([0, M], dtype=torch.int32, device="cuda")
+    leaves = [v.requires_grad_() for v in (rows, weight, bias)]
+    y = ska.grouped_linear(rows, weight, offsets, bias)
+    dr, dw, db = torch.autograd.grad(y, leaves, grad)
+    r, w, c, d = (v.detach().double() for v in (
+        rows, weight[0], bias[0], grad))
+    R, W, C, D = (v.abs() for v in (r, w, c, d))
+    check_there(y.detach(), r @ w.t() + c, R @ W.t() + C, F + 1)
+    check_there(dr, d @ w, D @ W, N)
+    check_there(dw[0], d.t() @ r, D.t() @ R, M)
+    check_there(db[0], d.sum(0), D.sum(0), M)
+
+
 @pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("dtype", TYPES, ids=SHORT.get)
 def test_grouped_linear_keeps_groups_apart(device, dtype):
