@@ -2004,6 +2004,9 @@ void product_launch(Product p, at::TensorOptions opt) {
   //            65536, 64,  256, 1024:   99 /  78 /   70 /   79
   //            28273, 179, 2072,  84:   84 /  59 /   59 /   61
   //            60000, 300,  720,  40:   60 /  45 /   42 /   31
+  //             8198, 48,  768,  768:   29 /  27 /      /   31
+  //            16384, 64, 1024, 1024:   81 /  75 /      /   92
+  //            32768, 64, 1024, 1024:  116 / 116 /      /  151
   //
   // One tile of c at a time, where enough blocks share a CU (us with two / one
   // at 128^2): forward 28273, 179, 2072, 84: 93 / 71; 8192, 8, 1024, 1024:
@@ -2034,8 +2037,9 @@ void product_launch(Product p, at::TensorOptions opt) {
            (MODE == kDWeight ? each : p.C) > 2 * KS;
   };
   if constexpr (MODE == kDWeight) {
-    // 256^2 where that fills the card and its edges waste less than a third
-    const bool large = p.G * tiles(256) >= 400 &&
+    // 256^2 where that fills the card, its edges waste less than a third and
+    // the rows of a group outlast a block's first loads
+    const bool large = each >= 512 && p.G * tiles(256) >= 400 &&
                        tiles(256) * 65536 * 3 <= 4l * p.M * p.N;
     const bool middle = p.M > 64 && p.N > 64 && p.G * tiles(128) >= 256;
     if (large && async && !kWide) {
