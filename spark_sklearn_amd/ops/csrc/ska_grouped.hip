@@ -346,7 +346,7 @@ void sort_launch(const I* ids, int M, int G, int* offsets, int* slots,
                  int* order, at::TensorOptions opt) {
   hipStream_t s = stream_now();
   // us for 100 / 1000 / 2048 entries in one block, and in the passes below:
-  // 64 groups 7 / 14 / 20, and 13; 4096 groups 9 / 16 / 23, and 28
+  // 64 groups 7 / 14 / 20, and 13; 4096 groups 9 / 16 / 23, and 21
   if (M <= (G < 2048 ? kSmallEntries / 2 : kSmallEntries) &&
       G <= kSmallGroups) {
     int size = 2;
@@ -360,7 +360,10 @@ void sort_launch(const I* ids, int M, int G, int* offsets, int* slots,
   }
   int bits = 1;
   while ((G >> bits) != 0) ++bits;  // keys are 0 .. G
-  const bool one = G + 1 <= kBins;
+  // One pass has as many counters a block as groups.  us for one / two:
+  // 4096 groups, 25000 entries 30 / 27, 100000 31 / 38; 6000 groups, 100000
+  // 44 / 39, 300000 48 / 50; 8000 groups, 3000 entries 46 / 22
+  const bool one = G + 1 <= kBins && M >= 40l * (G - 2750);
   const int digit = one ? bits : (bits + 1) / 2;
   const int mask = (1 << digit) - 1;
   const int bins = one ? G + 1 : 1 << digit;

@@ -99,7 +99,9 @@ def test_group_rows(device, itype, T, k, G, case):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("M,G", [(3_000_000, 1000), (2_300_001, 100_000)])
+@pytest.mark.parametrize("M,G", [
+    (3_000_000, 1000), (2_300_001, 100_000), (60_001, 4096), (10_000, 3000),
+    (9_999, 3000), (217_640, 8191), (250_007, 8191), (250_007, 8192)])
 def test_group_rows_many(M, G):
     ids = ids_of("dropped", M, 1, G)
     offsets, slots, order = plan64(ids, G)
