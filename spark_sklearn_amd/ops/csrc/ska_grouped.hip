@@ -14,7 +14,6 @@
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <hip/hip_runtime.h>
-#include <torch/csrc/autograd/functions/basic_ops.h>
 
 #include <algorithm>
 #include <tuple>
@@ -2216,14 +2215,29 @@ bool wants(const Maybe& t) { return t && wants(*t); }
 
 at::Tensor defined_or_none(const Maybe& t) { return t ? *t : at::Tensor(); }
 
-// The kernels' gradients have no gradients of their own: a second
-// differentiation is an error, and not zero.
-variable_list once(variable_list grads) {
-  if (!at::GradMode::is_enabled()) return grads;
-  auto stop = std::make_shared<torch::autograd::DelayedError>(
-      "grouped-row operators can be differentiated once only",
-      (int64_t)grads.size());
-  return (*stop)(std::move(grads));
+// The kernels' gradients have no gradients of their own.  Where a graph of the
+// backward pass is asked for, a gradient gets a node between itself and the two
+// tensors it is a product of, the incoming gradient and a saved operand: a
+// second differentiation that comes through it is an error, whatever else the
+// loss holds, and one that does not is none of its business.
+template <typename Make>
+struct OnceFunction : torch::autograd::Function<OnceFunction<Make>> {
+  static at::Tensor forward(AutogradContext*, const Make& make,
+                            const at::Tensor&, const at::Tensor&) {
+    return make();
+  }
+  static variable_list backward(AutogradContext*, variable_list) {
+    TORCH_CHECK(false,
+                "grouped-row operators can be differentiated once only");
+  }
+};
+
+template <typename Make>
+at::Tensor once(const at::Tensor& grad, const at::Tensor& operand,
+                const Make& make) {
+  if (!at::GradMode::is_enabled()) return make();
+  return OnceFunction<Make>::apply(make, grad,
+                                   operand.defined() ? operand : grad);
 }
 
 struct GatherFunction : torch::autograd::Function<GatherFunction> {
@@ -2236,8 +2250,10 @@ struct GatherFunction : torch::autograd::Function<GatherFunction> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     auto saved = ctx->get_saved_variables();
     // a row's gradient is the sum over its places
-    auto dx = combine_rows(grads[0], saved[0], saved[1], c10::nullopt);
-    return once({dx, at::Tensor(), at::Tensor()});
+    auto dx = once(grads[0], at::Tensor(), [&] {
+      return combine_rows(grads[0], saved[0], saved[1], c10::nullopt);
+    });
+    return {dx, at::Tensor(), at::Tensor()};
   }
 };
 
@@ -2254,16 +2270,30 @@ struct CombineFunction : torch::autograd::Function<CombineFunction> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     auto saved = ctx->get_saved_variables();
+    const bool need_rows =
+        ctx->saved_data["rows"].toBool() && ctx->needs_input_grad(0);
     const bool need_weights =
         ctx->saved_data["weights"].toBool() && ctx->needs_input_grad(3);
-    auto got = combine_rows_backward(
-        grads[0], need_weights ? saved[0] : grads[0], saved[1], saved[2],
-        saved[3].defined() ? Maybe(saved[3]) : Maybe(),
-        ctx->saved_data["rows"].toBool() && ctx->needs_input_grad(0),
-        need_weights);
-    return once({defined_or_none(std::get<0>(got)), at::Tensor(),
-                 at::Tensor(), defined_or_none(std::get<1>(got)),
-                 at::Tensor(), at::Tensor()});
+    const Maybe weights = saved[3].defined() ? Maybe(saved[3]) : Maybe();
+    auto both = [&](bool rows, bool dots) {
+      return combine_rows_backward(grads[0], dots ? saved[0] : grads[0],
+                                   saved[1], saved[2], weights, rows, dots);
+    };
+    at::Tensor drows, dw;
+    if (!at::GradMode::is_enabled()) {  // in one pass
+      auto got = both(need_rows, need_weights);
+      drows = defined_or_none(std::get<0>(got));
+      dw = defined_or_none(std::get<1>(got));
+    } else {
+      if (need_rows)
+        drows = once(grads[0], saved[3],
+                     [&] { return *std::get<0>(both(true, false)); });
+      if (need_weights)
+        dw = once(grads[0], saved[0],
+                  [&] { return *std::get<1>(both(false, true)); });
+    }
+    return {drows, at::Tensor(), at::Tensor(), dw, at::Tensor(),
+            at::Tensor()};
   }
 };
 
@@ -2283,20 +2313,34 @@ struct LinearFunction : torch::autograd::Function<LinearFunction> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     auto saved = ctx->get_saved_variables();
-    at::Tensor drows;
+    at::Tensor drows, dweight, dbias;
     if (ctx->saved_data["rows"].toBool() && ctx->needs_input_grad(0))
-      drows = grouped_linear_drows(grads[0], saved[1], saved[2]);
-    std::tuple<Maybe, Maybe> got;
+      drows = once(grads[0], saved[1], [&] {
+        return grouped_linear_drows(grads[0], saved[1], saved[2]);
+      });
     const bool need_weight =
         ctx->saved_data["weight"].toBool() && ctx->needs_input_grad(1);
     const bool need_bias =
         ctx->saved_data["bias"].toBool() && ctx->needs_input_grad(3);
-    if (need_weight || need_bias)
-      got = grouped_linear_dweight(grads[0], saved[0], saved[2], need_weight,
-                                   need_bias);
-    return once({drows, defined_or_none(std::get<0>(got)), at::Tensor(),
-                 defined_or_none(std::get<1>(got)), at::Tensor(),
-                 at::Tensor(), at::Tensor()});
+    auto both = [&](bool weight, bool bias) {
+      return grouped_linear_dweight(grads[0], saved[0], saved[2], weight,
+                                    bias);
+    };
+    if (!at::GradMode::is_enabled()) {  // in one pass
+      std::tuple<Maybe, Maybe> got;
+      if (need_weight || need_bias) got = both(need_weight, need_bias);
+      dweight = defined_or_none(std::get<0>(got));
+      dbias = defined_or_none(std::get<1>(got));
+    } else {
+      if (need_weight)
+        dweight = once(grads[0], saved[0],
+                       [&] { return *std::get<0>(both(true, false)); });
+      if (need_bias)
+        dbias = once(grads[0], at::Tensor(),
+                     [&] { return *std::get<1>(both(false, true)); });
+    }
+    return {drows,        dweight,      at::Tensor(), dbias,
+            at::Tensor(), at::Tensor(), at::Tensor()};
   }
 };
 

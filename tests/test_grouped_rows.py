@@ -932,3 +932,75 @@ def test_refuses_mixed_devices():
         ska.grouped_linear(rows.cuda(), weight, plan.offsets.cuda())
     with pytest.raises(TypeError):
         ska.gather_rows(x.cuda().double(), plan)
+
+
+# -- derivatives of derivatives -----------------------------------------------
+
+def second_orders(device):
+    """(leaf, loss) pairs whose losses hold a gradient and, beside it, a term
+    that is differentiable once: the error may not be passed by."""
+    for i in range(4):
+        for where in (0, 1, 2):
+            x, ids, weight, bias, w, dy = chain_data(device, T=20)
+            leaves = [v.detach().requires_grad_(j == i)
+                      for j, v in enumerate((x, weight, bias, w))]
+            y = chain(leaves[0], ids, weight.shape[0], *leaves[1:])
+            g, = torch.autograd.grad((y * y).sum(), leaves[i],
+                                     create_graph=True)
+            assert g.requires_grad
+            yield leaves[i], (y.sum() + (g * g).sum(),
+                              leaves[i].sum() + g.sum(),
+                              y.square().sum() + g.sum())[where]
+
+
+@pytest.mark.gpu
+def test_second_derivatives_raise_on_the_gpu():
+    for leaf, loss in second_orders("cuda"):
+        with pytest.raises(RuntimeError, match="once only"):
+            torch.autograd.grad(loss, leaf, retain_graph=True)
+        with pytest.raises(RuntimeError, match="once only"):
+            loss.backward()
+
+
+@pytest.mark.gpu
+def test_a_gradients_other_sources_raise_on_the_gpu():
+    """A gradient is linear in the incoming one and in the saved operand; it
+    raises for these and is a constant for the rest."""
+    x, ids, weight, bias, w, dy = chain_data("cuda", T=20)
+    plan = ska.group_rows(ids, weight.shape[0])
+    rows = ska.gather_rows(x, plan).requires_grad_()
+    weight.requires_grad_()
+    bias.requires_grad_()
+    out = ska.grouped_linear(rows, weight, plan.offsets, bias)
+    drows, dweight, dbias = torch.autograd.grad(
+        out.sum(), [rows, weight, bias], create_graph=True)
+    for got, raises, constant in ((drows, weight, rows),
+                                  (dweight, rows, weight)):
+        with pytest.raises(RuntimeError, match="once only"):
+            torch.autograd.grad(raises.sum() + got.sum(), raises,
+                                retain_graph=True)
+        plain, = torch.autograd.grad(constant.sum() + got.sum(), constant,
+                                     retain_graph=True)
+        assert bool((plain == 1).all())
+    assert not dbias.requires_grad
+    w.requires_grad_()
+    y = ska.combine_rows(rows, plan, w)
+    drows, dw = torch.autograd.grad(y.sum(), [rows, w], create_graph=True)
+    for got, raises, constant in ((drows, w, rows), (dw, rows, w)):
+        with pytest.raises(RuntimeError, match="once only"):
+            torch.autograd.grad(raises.sum() + got.sum(), raises,
+                                retain_graph=True)
+        plain, = torch.autograd.grad(constant.sum() + got.sum(), constant,
+                                     retain_graph=True)
+        assert bool((plain == 1).all())
+
+
+@pytest.mark.gpu
+def test_gradients_are_the_same_with_a_graph_of_them():
+    for i in range(2):
+        x, ids, weight, bias, w, dy = chain_data("cuda", T=333)
+        leaves = [v.requires_grad_() for v in (x, weight, bias, w)]
+        y = chain(leaves[0], ids, weight.shape[0], *leaves[1:])
+        a = torch.autograd.grad(y, leaves, dy, retain_graph=True)
+        b = torch.autograd.grad(y, leaves, dy, create_graph=True)
+        assert all(torch.equal(u, v) for u, v in zip(a, b))
