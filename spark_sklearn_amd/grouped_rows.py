@@ -137,9 +137,22 @@ def _make_reference():
     from types import SimpleNamespace
 
     import torch
-    from torch.autograd.function import once_differentiable
 
     from .models import _grouped_ref as ref
+
+    class Once(torch.autograd.Function):
+        """A gradient between the tensors it is a product of, the incoming
+        gradient and a saved operand: a second differentiation that comes
+        through it is an error, whatever else the loss holds."""
+
+        @staticmethod
+        def forward(ctx, make, grad, operand=None):
+            return make()
+
+        @staticmethod
+        def backward(ctx, grad):
+            raise RuntimeError(
+                "grouped-row operators can be differentiated once only")
 
     class Gather(torch.autograd.Function):
         @staticmethod
@@ -148,11 +161,10 @@ def _make_reference():
             return ref.gather_rows_ref(x, offsets, slots)
 
         @staticmethod
-        @once_differentiable
         def backward(ctx, grad):
             # a row's gradient is the sum over its places
-            return ref.combine_rows_ref(grad, *ctx.saved_tensors,
-                                        None), None, None
+            return Once.apply(lambda: ref.combine_rows_ref(
+                grad, *ctx.saved_tensors, None), grad), None, None
 
     class Combine(torch.autograd.Function):
         @staticmethod
@@ -161,11 +173,17 @@ def _make_reference():
             return ref.combine_rows_ref(rows, offsets, slots, weights)
 
         @staticmethod
-        @once_differentiable
         def backward(ctx, grad):
-            drows, dw = ref.combine_rows_backward_ref(
-                grad, *ctx.saved_tensors, ctx.needs_input_grad[0],
-                ctx.needs_input_grad[3])
+            rows, offsets, slots, weights = ctx.saved_tensors
+            drows = dw = None
+            if ctx.needs_input_grad[0]:
+                drows = Once.apply(lambda: ref.combine_rows_backward_ref(
+                    grad, rows, offsets, slots, weights, True, False)[0],
+                    grad, weights)
+            if ctx.needs_input_grad[3]:
+                dw = Once.apply(lambda: ref.combine_rows_backward_ref(
+                    grad, rows, offsets, slots, weights, False, True)[1],
+                    grad, rows)
             return drows, None, None, dw
 
     class Linear(torch.autograd.Function):
@@ -175,15 +193,18 @@ def _make_reference():
             return ref.grouped_linear_ref(rows, weight, offsets, bias)
 
         @staticmethod
-        @once_differentiable
         def backward(ctx, grad):
             rows, weight, offsets = ctx.saved_tensors
-            drows = None
+            drows = dweight = dbias = None
             if ctx.needs_input_grad[0]:
-                drows = ref.grouped_linear_drows_ref(grad, weight, offsets)
-            dweight, dbias = ref.grouped_linear_dweight_ref(
-                grad, rows, offsets, ctx.needs_input_grad[1],
-                ctx.needs_input_grad[3])
+                drows = Once.apply(lambda: ref.grouped_linear_drows_ref(
+                    grad, weight, offsets), grad, weight)
+            if ctx.needs_input_grad[1]:
+                dweight = Once.apply(lambda: ref.grouped_linear_dweight_ref(
+                    grad, rows, offsets, True, False)[0], grad, rows)
+            if ctx.needs_input_grad[3]:
+                dbias = Once.apply(lambda: ref.grouped_linear_dweight_ref(
+                    grad, rows, offsets, False, True)[1], grad)
             return drows, dweight, None, dbias
 
     return SimpleNamespace(

@@ -1004,3 +1004,20 @@ def test_gradients_are_the_same_with_a_graph_of_them():
         a = torch.autograd.grad(y, leaves, dy, retain_graph=True)
         b = torch.autograd.grad(y, leaves, dy, create_graph=True)
         assert all(torch.equal(u, v) for u, v in zip(a, b))
+
+
+def test_second_derivatives_raise_on_the_cpu():
+    for leaf, loss in second_orders("cpu"):
+        with pytest.raises(RuntimeError, match="once only"):
+            torch.autograd.grad(loss, leaf, retain_graph=True)
+        with pytest.raises(RuntimeError, match="once only"):
+            loss.backward()
+
+
+def test_gradients_are_the_same_with_a_graph_of_them_on_the_cpu():
+    x, ids, weight, bias, w, dy = chain_data("cpu", T=99)
+    leaves = [v.requires_grad_() for v in (x, weight, bias, w)]
+    y = chain(leaves[0], ids, weight.shape[0], *leaves[1:])
+    a = torch.autograd.grad(y, leaves, dy, retain_graph=True)
+    b = torch.autograd.grad(y, leaves, dy, create_graph=True)
+    assert all(torch.equal(u, v) for u, v in zip(a, b))
