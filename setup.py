@@ -6,6 +6,7 @@ The .so lands next to the package (spark_sklearn_amd/_hip_ops*.so) so it
 travels with the repo snapshot to the GPU box (no JIT cache dependence).
 """
 
+import glob
 import os
 import sys
 
@@ -15,10 +16,20 @@ os.environ.setdefault("PYTORCH_ROCM_ARCH", "gfx950")
 
 from torch.utils.cpp_extension import BuildExtension, CUDAExtension  # noqa: E402
 
+HEADERS = ["spark_sklearn_amd/ops/csrc/ska_rows.h"]
+
+# ninja knows nothing of the headers that HIP sources include: objects that
+# are older than one of them are built again
+newest = max(os.path.getmtime(h) for h in HEADERS)
+for built in glob.glob("build/temp*/spark_sklearn_amd/ops/csrc/*.o"):
+    if os.path.getmtime(built) < newest:
+        os.remove(built)
+
 ext = CUDAExtension(
     name="spark_sklearn_amd._hip_ops",
     sources=["spark_sklearn_amd/ops/csrc/ska_ops.hip",
              "spark_sklearn_amd/ops/csrc/ska_grouped.hip"],
+    depends=HEADERS,
     extra_compile_args={
         "cxx": ["-O3", "-std=c++17"],
         # packed fp32 instructions stay off: hipcc makes them from ordinary

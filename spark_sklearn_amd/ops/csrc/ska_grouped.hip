@@ -19,6 +19,8 @@
 #include <tuple>
 #include <type_traits>
 
+#include "ska_rows.h"
+
 namespace {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -53,20 +55,6 @@ __device__ __forceinline__ int clampi(int v, int lo, int hi) {
 template <typename I>
 __device__ __forceinline__ int key_of(I id, int G) {
   return (id < 0 || id >= (I)G) ? G : (int)id;
-}
-
-// The first position in keys[0, n) whose key is not below g.
-template <typename K>
-__device__ __forceinline__ int lower_bound(const K* keys, int n, K g) {
-  int lo = 0, hi = n;
-  while (lo < hi) {
-    int mid = (lo + hi) >> 1;
-    if (keys[mid] < g)
-      lo = mid + 1;
-    else
-      hi = mid;
-  }
-  return lo;
 }
 
 constexpr int kSmallEntries = 2048;
@@ -120,7 +108,7 @@ __global__ __launch_bounds__(1024) void sort_small_kernel(
     slots[entry] = i;
   }
   for (int g = tid; g <= G; g += threads)
-    offsets[g] = lower_bound(item, M, (unsigned)g * kSmallEntries);
+    offsets[g] = ska::lower_bound(item, M, (unsigned)g * kSmallEntries);
 }
 
 // Many entries: passes over a digit of the key, low digit first.  One pass
@@ -337,7 +325,7 @@ __global__ void sort_offsets_kernel(const int* __restrict__ keys, int M,
                                     int G, int* __restrict__ offsets) {
   for (long g = (long)blockIdx.x * blockDim.x + threadIdx.x; g <= G;
        g += (long)gridDim.x * blockDim.x)
-    offsets[g] = lower_bound(keys, M, (int)g);
+    offsets[g] = ska::lower_bound(keys, M, (int)g);
 }
 
 template <typename I>

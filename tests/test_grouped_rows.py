@@ -1021,3 +1021,22 @@ def test_gradients_are_the_same_with_a_graph_of_them_on_the_cpu():
     a = torch.autograd.grad(y, leaves, dy, retain_graph=True)
     b = torch.autograd.grad(y, leaves, dy, create_graph=True)
     assert all(torch.equal(u, v) for u, v in zip(a, b))
+
+
+# -- row numbers near 2^31 ----------------------------------------------------
+
+@pytest.mark.gpu
+def test_group_rows_beyond_half_of_the_row_numbers():
+    """More than 2^30 entries in more groups than one pass takes: entry i has
+    the group i % G, so that its place is known."""
+    M, G = (1 << 30) + 12345, 10007
+    ids = torch.arange(M, dtype=torch.int32, device="cuda").remainder_(G)
+    plan = ska.group_rows(ids, G)
+    g = torch.arange(G + 1, device="cuda")
+    offsets = g * (M // G) + g.clamp(max=M % G)
+    assert torch.equal(plan.offsets, offsets.int())
+    for lo in range(0, M, 1 << 28):
+        i = torch.arange(lo, min(M, lo + (1 << 28)), device="cuda")
+        place = offsets[i % G] + i // G
+        assert torch.equal(plan.slots[lo:lo + (1 << 28)], place.int())
+        assert torch.equal(plan.order[place], i.int())
