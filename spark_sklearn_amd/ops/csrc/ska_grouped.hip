@@ -1281,7 +1281,7 @@ __device__ __forceinline__ bool find_job(const Product& p, int tile,
       job.group = seg.group;
       first = seg.first;
       start = seg.start;
-      job.steps = min(seg.end - first, 1 << p.shift);
+      job.steps = ska::part_end(first, seg.end, p.shift) - first;
       job.parted = seg.end - seg.start > (1 << p.shift);
     } else {
       job.group = unit;
@@ -1573,7 +1573,7 @@ __global__ __launch_bounds__(256) void finish_kernel(Product p) {
   const int g = blockIdx.x;
   const int start = edge(p.offsets, g, p.G, p.C);
   const int end = edge(p.offsets, g + 1, p.G, p.C);
-  const int count = (end - start + (1 << p.shift) - 1) >> p.shift;
+  const int count = ska::part_count(start, end, p.shift);
   if (count == 1) return;
   const long size = (long)p.M * p.N;
   const long unit = part_place(start, p.shift);
@@ -1740,7 +1740,7 @@ __global__ __launch_bounds__(256) void narrow_dweight_kernel(Product p) {
   constexpr int BF = 4 / KW * 64;
   const Segment seg = find_segment(p.offsets, p.G, p.C, blockIdx.x, p.shift);
   if (seg.first >= seg.end || seg.group >= p.G) return;
-  const int end = min(seg.end, seg.first + (1 << p.shift));
+  const int end = ska::part_end(seg.first, seg.end, p.shift);
   const bool parted = seg.end - seg.start > (1 << p.shift);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;

@@ -20,4 +20,14 @@ constexpr int lower_bound(const Keys& keys, int n, K g) {
   return lo;
 }
 
+// Rows first .. last - 1 in parts of 2^shift: how many parts there are, and
+// where the one that begins at `at` ends.
+constexpr int part_count(int first, int last, int shift) {
+  return first < last ? ((last - first - 1) >> shift) + 1 : 0;
+}
+constexpr int part_end(int at, int last, int shift) {
+  const int rest = last - at, whole = 1 << shift;
+  return at + (rest < whole ? rest : whole);
+}
+
 }  // namespace ska

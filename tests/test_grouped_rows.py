@@ -1040,3 +1040,23 @@ def test_group_rows_beyond_half_of_the_row_numbers():
         place = offsets[i % G] + i // G
         assert torch.equal(plan.slots[lo:lo + (1 << 28)], place.int())
         assert torch.equal(plan.order[place], i.int())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16],
+                         ids=SHORT.get)
+def test_gradients_of_a_group_of_all_row_numbers(dtype):
+    """As many rows as there may be, in one group.  Sums of ones: whole
+    numbers, exact in 32 bits up to 2^24 and in fewer than 2^12 parts, each of
+    whose additions is off by half a step of the sum so far, 2^-24 of it."""
+    M = 2 ** 31 - 65537
+    rows = torch.ones(M, 1, dtype=dtype, device="cuda")
+    weight = torch.ones(1, 1, 1, dtype=dtype, device="cuda",
+                        requires_grad=True)
+    bias = torch.ones(1, 1, dtype=dtype, device="cuda", requires_grad=True)
+    offsets = torch.tensor([0, M], dtype=torch.int32, device="cuda")
+    y = ska.grouped_linear(rows, weight, offsets, bias)
+    assert bool((y[-70000:] == 2).all())
+    dweight, dbias = torch.autograd.grad(y, [weight, bias], rows)
+    tol = M * (2.0 ** -12 + torch.finfo(dtype).eps / 2)
+    assert abs(float(dweight) - M) <= tol and abs(float(dbias) - M) <= tol

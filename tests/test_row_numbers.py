@@ -33,6 +33,14 @@ extern "C" int64_t find(int64_t n, int64_t each, int64_t g) {
     return -1;
   }
 }
+
+extern "C" int64_t count(int64_t first, int64_t last, int64_t shift) {
+  return ska::part_count((int)first, (int)last, (int)shift);
+}
+
+extern "C" int64_t end(int64_t at, int64_t last, int64_t shift) {
+  return ska::part_end((int)at, (int)last, (int)shift);
+}
 """
 
 
@@ -49,7 +57,7 @@ def host(tmp_path_factory):
         [compiler, "-std=c++17", "-O1", "-fwrapv", "-shared", "-fPIC",
          "-I", CSRC, str(source), "-o", str(built)], check=True)
     lib = ctypes.CDLL(str(built))
-    for name in ("find",):
+    for name in ("find", "count", "end"):
         getattr(lib, name).restype = ctypes.c_int64
     return lib
 
@@ -63,3 +71,25 @@ def test_lower_bound(host, n, groups):
                      n // each}):
         at = host.find(*(ctypes.c_int64(v) for v in (n, each, g)))
         assert at == min(n, g * each)
+
+
+@pytest.mark.parametrize("shift", [6, 8, 9, 16, 20, 22, 30])
+@pytest.mark.parametrize("first,last", [
+    (0, 0), (0, 1), (5, 5), (3, 1000), (0, 2 ** 30), (1, 2 ** 30 + 2),
+    (0, MOST), (1, MOST), (12345, MOST), (MOST - 70000, MOST),
+    (MOST - 1, MOST), (MOST, MOST)])
+def test_parts(host, first, last, shift):
+    size = 1 << shift
+    count = host.count(*(ctypes.c_int64(v) for v in (first, last, shift)))
+    assert count == -(-(last - first) // size)
+    for part in (0, 1, count // 2, count - 2, count - 1):
+        if not 0 <= part < count:
+            continue
+        at = first + part * size
+        end = host.end(*(ctypes.c_int64(v) for v in (at, last, shift)))
+        assert end == min(last, at + size)
+
+
+def test_a_group_that_ends_before_it_begins_has_no_parts(host):
+    """As offsets that decrease would have it."""
+    assert host.count(*(ctypes.c_int64(v) for v in (900, 100, 8))) == 0
