@@ -759,7 +759,16 @@ at::Tensor packed_rows(const at::Tensor& t) {
   return fits ? t : t.contiguous();
 }
 
+// The kernels have no forward-mode derivatives, and a tensor that came back
+// without its tangent would pass for a constant.
+void check_plain(const char* name, const at::Tensor& t) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!t._fw_grad(/*level=*/0).defined(), name,
+                              " has a tangent: grouped-row operators have no "
+                              "forward-mode derivatives");
+}
+
 void check_rows(const char* name, const at::Tensor& t) {
+  check_plain(name, t);
   TORCH_CHECK_VALUE(t.is_cuda(), name, " must be on a GPU, got ", t.device());
   TORCH_CHECK_TYPE(t.dtype() == at::kFloat || t.dtype() == at::kBFloat16 ||
                        t.dtype() == at::kHalf,
@@ -782,6 +791,7 @@ void check_ints(const char* name, const at::Tensor& t,
 
 void check_same(const char* name, const at::Tensor& t,
                 const at::Tensor& rows) {
+  check_plain(name, t);
   TORCH_CHECK_TYPE(t.dtype() == rows.dtype(), name, " must be ", rows.dtype(),
                    " like the rows, got ", t.dtype());
   TORCH_CHECK_VALUE(t.device() == rows.device(), name, " is on ", t.device(),
@@ -2236,6 +2246,7 @@ struct GatherFunction : torch::autograd::Function<GatherFunction> {
     return gather_rows(x, offsets, slots);
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    check_plain("the gradient", grads[0]);
     auto saved = ctx->get_saved_variables();
     // a row's gradient is the sum over its places
     auto dx = once(grads[0], at::Tensor(), [&] {
@@ -2257,6 +2268,7 @@ struct CombineFunction : torch::autograd::Function<CombineFunction> {
     return combine_rows(rows, offsets, slots, weights);
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    check_plain("the gradient", grads[0]);
     auto saved = ctx->get_saved_variables();
     const bool need_rows =
         ctx->saved_data["rows"].toBool() && ctx->needs_input_grad(0);
@@ -2300,6 +2312,7 @@ struct LinearFunction : torch::autograd::Function<LinearFunction> {
     return grouped_linear(rows, weight, offsets, bias);
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    check_plain("the gradient", grads[0]);
     auto saved = ctx->get_saved_variables();
     at::Tensor drows, dweight, dbias;
     if (ctx->saved_data["rows"].toBool() && ctx->needs_input_grad(0))
@@ -2351,6 +2364,7 @@ at::Tensor combine_rows_checked(const at::Tensor& rows,
   TORCH_CHECK_VALUE(plan.slots.numel() == rows.size(0), "rows has ",
                     rows.size(0), " rows, the plan ", plan.slots.numel());
   if (weights) {
+    check_plain("weights", *weights);
     TORCH_CHECK_TYPE(
         weights->dtype() == at::kFloat || weights->dtype() == rows.dtype(),
         "weights must be float32 or ", rows.dtype(), ", got ",

@@ -1060,3 +1060,38 @@ def test_gradients_of_a_group_of_all_row_numbers(dtype):
     dweight, dbias = torch.autograd.grad(y, [weight, bias], rows)
     tol = M * (2.0 ** -12 + torch.finfo(dtype).eps / 2)
     assert abs(float(dweight) - M) <= tol and abs(float(dbias) - M) <= tol
+
+
+# -- calls that the kernels refuse ----------------------------------------------
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_forward_mode_raises(device):
+    """A tangent is refused, in the inputs and in an incoming gradient: it
+    would come back as none, which stands for zero."""
+    import torch.autograd.forward_ad as fw
+
+    x, ids, weight, bias, w, dy = chain_data(device, T=20)
+    G = weight.shape[0]
+    plan = ska.group_rows(ids, G)
+    rows = ska.gather_rows(x, plan)
+    out = ska.grouped_linear(rows, weight, plan.offsets, bias)
+    with fw.dual_level():
+        def dual(v):
+            return fw.make_dual(v.detach().clone(), torch.ones_like(v))
+
+        for call in (
+                lambda: ska.gather_rows(dual(x), plan),
+                lambda: ska.grouped_linear(dual(rows), weight, plan.offsets),
+                lambda: ska.grouped_linear(rows, dual(weight), plan.offsets),
+                lambda: ska.grouped_linear(rows, weight, plan.offsets,
+                                           dual(bias)),
+                lambda: ska.combine_rows(dual(out), plan, w),
+                lambda: ska.combine_rows(out, plan, dual(w))):
+            with pytest.raises(NotImplementedError):
+                call()
+        for i in range(4):
+            leaves = [v.detach().requires_grad_(j == i)
+                      for j, v in enumerate((x, weight, bias, w))]
+            y = chain(leaves[0], ids, G, *leaves[1:])
+            with pytest.raises(NotImplementedError):
+                torch.autograd.grad(y, leaves[i], dual(dy))
