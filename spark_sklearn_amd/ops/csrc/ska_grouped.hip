@@ -10,6 +10,7 @@
 // No kernel trusts the values of offsets and slots for its addresses: an
 // offset is clamped to the rows there are, a slot outside them is skipped.
 
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -38,6 +39,20 @@ void check_launch() {
 constexpr int64_t kMaxGroups = (1 << 24) - 1;
 constexpr int64_t kMaxWidth = (1 << 21) - 1;
 constexpr int64_t kMaxRows = (1ll << 31) - (1 << 16) - 1;
+
+// The kernels have no forward-mode derivatives, and a tensor that came back
+// without its tangent would pass for a constant.
+void check_plain(const char* name, const at::Tensor& t) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!t._fw_grad(/*level=*/0).defined(), name,
+                              " has a tangent: grouped-row operators have no "
+                              "forward-mode derivatives");
+}
+
+// A trace would record the allocations of the outputs and not the kernels.
+void check_not_traced() {
+  TORCH_CHECK(!torch::jit::tracer::isTracing(),
+              "grouped-row operators cannot be traced on a GPU");
+}
 
 template <typename T>
 __device__ __forceinline__ float to_f(T v) {
@@ -415,6 +430,7 @@ void sort_launch(const I* ids, int M, int G, int* offsets, int* slots,
 
 std::tuple<at::Tensor, at::Tensor, at::Tensor> group_rows(
     const at::Tensor& ids_in, int64_t n_groups) {
+  check_not_traced();
   TORCH_CHECK_VALUE(ids_in.is_cuda(), "ids must be on a GPU, got ",
                     ids_in.device());
   TORCH_CHECK_TYPE(ids_in.dtype() == at::kInt || ids_in.dtype() == at::kLong,
@@ -757,14 +773,6 @@ at::Tensor packed_rows(const at::Tensor& t) {
       (t.size(0) == 1 ||
        (t.stride(0) >= t.size(1) && t.stride(0) < (1 << 22)));
   return fits ? t : t.contiguous();
-}
-
-// The kernels have no forward-mode derivatives, and a tensor that came back
-// without its tangent would pass for a constant.
-void check_plain(const char* name, const at::Tensor& t) {
-  TORCH_CHECK_NOT_IMPLEMENTED(!t._fw_grad(/*level=*/0).defined(), name,
-                              " has a tangent: grouped-row operators have no "
-                              "forward-mode derivatives");
 }
 
 void check_rows(const char* name, const at::Tensor& t) {
@@ -2348,6 +2356,7 @@ struct LinearFunction : torch::autograd::Function<LinearFunction> {
 // The entry points: checks, then with or without a place in the graph.
 at::Tensor gather_rows_checked(const at::Tensor& x, const at::Tensor& offsets,
                                const at::Tensor& slots) {
+  check_not_traced();
   check_rows("x", x);
   const Plan plan = check_plan(x, offsets, slots);
   TORCH_CHECK_VALUE(plan.slots.size(0) == x.size(0), "x has ", x.size(0),
@@ -2359,6 +2368,7 @@ at::Tensor gather_rows_checked(const at::Tensor& x, const at::Tensor& offsets,
 at::Tensor combine_rows_checked(const at::Tensor& rows,
                                 const at::Tensor& offsets,
                                 const at::Tensor& slots, Maybe weights) {
+  check_not_traced();
   check_rows("rows", rows);
   const Plan plan = check_plan(rows, offsets, slots);
   TORCH_CHECK_VALUE(plan.slots.numel() == rows.size(0), "rows has ",
@@ -2386,6 +2396,7 @@ at::Tensor combine_rows_checked(const at::Tensor& rows,
 at::Tensor grouped_linear_checked(const at::Tensor& rows,
                                   const at::Tensor& weight_in,
                                   const at::Tensor& offsets_in, Maybe bias) {
+  check_not_traced();
   check_rows("rows", rows);
   check_ints("offsets", offsets_in, rows);
   TORCH_CHECK_VALUE(weight_in.dim() == 3,
@@ -2423,6 +2434,7 @@ at::Tensor grouped_linear_checked(const at::Tensor& rows,
 std::tuple<Maybe, Maybe> grouped_linear_dweight_checked(
     const at::Tensor& dy, const at::Tensor& rows, const at::Tensor& offsets,
     bool need_weight, bool need_bias) {
+  check_not_traced();
   check_rows("dy", dy);
   check_rows("rows", rows);
   check_same("dy", dy, rows);

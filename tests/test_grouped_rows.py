@@ -1095,3 +1095,33 @@ def test_forward_mode_raises(device):
             y = chain(leaves[0], ids, G, *leaves[1:])
             with pytest.raises(NotImplementedError):
                 torch.autograd.grad(y, leaves[i], dual(dy))
+
+
+@pytest.mark.gpu
+def test_tracing_raises_on_the_gpu():
+    """A trace would hold the outputs' allocations and not the kernels."""
+    x, ids, weight, bias, w, dy = chain_data("cuda", T=20)
+    plan = ska.group_rows(ids, weight.shape[0])
+    out = ska.grouped_linear(ska.gather_rows(x, plan), weight, plan.offsets)
+    for call, given in (
+            (lambda v: ska.group_rows(v, 3).order, ids),
+            (lambda v: ska.gather_rows(v, plan), x),
+            (lambda v: ska.grouped_linear(v, weight, plan.offsets),
+             ska.gather_rows(x, plan)),
+            (lambda v: ska.combine_rows(v, plan), out)):
+        with pytest.raises(RuntimeError, match="traced"):
+            torch.jit.trace(call, given, check_trace=False)
+        call(given)
+
+
+def test_tracing_on_the_cpu_follows_its_inputs():
+    """The reference's calls are part of a trace."""
+    x, ids, weight, bias, w, dy = chain_data("cpu", T=20)
+    G = weight.shape[0]
+
+    def run(x, ids):
+        return chain(x, ids, G, weight, bias, w)
+
+    traced = torch.jit.trace(run, (x, ids), check_trace=False)
+    other = torch.as_tensor(ids_of("skewed", *ids.shape, G, seed=4))
+    assert torch.equal(traced(x + 1, other), run(x + 1, other))
