@@ -40,9 +40,30 @@ constexpr int64_t kMaxGroups = (1 << 24) - 1;
 constexpr int64_t kMaxWidth = (1 << 21) - 1;
 constexpr int64_t kMaxRows = (1ll << 31) - (1 << 16) - 1;
 
+// Whether the kernels can read a tensor: subclasses that wrap others, fake
+// tensors and zeros that are only noted as such have no memory behind them,
+// and what lies behind a functional tensor may be out of date.
+bool has_memory(const at::Tensor& t) {
+  return t.numel() == 0 ||
+         (t.layout() == at::kStrided && t.has_storage() &&
+          !t.key_set().has(c10::DispatchKey::Functionalize) &&
+          t.const_data_ptr() != nullptr);
+}
+
+// No address goes to a kernel but through here.  Inputs are checked on entry;
+// what torch makes of them, and outputs, may still be fakes (under a mode).
+template <typename T>
+T* ptr(const at::Tensor& t) {
+  TORCH_CHECK_TYPE(has_memory(t), "grouped-row operators take no tensors "
+                   "without memory (wrappers, fake tensors)");
+  return reinterpret_cast<T*>(t.data_ptr());
+}
+
 // The kernels have no forward-mode derivatives, and a tensor that came back
 // without its tangent would pass for a constant.
 void check_plain(const char* name, const at::Tensor& t) {
+  TORCH_CHECK_TYPE(has_memory(t), name, " must be a tensor with memory of its "
+                   "own (no wrapper or fake tensor, dense)");
   TORCH_CHECK_NOT_IMPLEMENTED(!t._fw_grad(/*level=*/0).defined(), name,
                               " has a tangent: grouped-row operators have no "
                               "forward-mode derivatives");
@@ -379,14 +400,14 @@ void sort_launch(const I* ids, int M, int G, int* offsets, int* slots,
     tile *= 2;
   const int blocks = (int)(((long)M + tile - 1) / tile);
   at::Tensor table = at::empty({(int64_t)bins * blocks + 2 * bins}, opt);
-  int* tab = table.data_ptr<int>();
+  int* tab = ptr<int>(table);
   int* total = tab + (long)bins * blocks;
   int* base = one ? offsets : total + bins;
   at::Tensor pairs;
   int *k0 = nullptr, *e0 = nullptr, *k1 = nullptr;
   if (!one) {
     pairs = at::empty({3 * (int64_t)M}, opt);
-    k0 = pairs.data_ptr<int>();
+    k0 = ptr<int>(pairs);
     e0 = k0 + M;
     k1 = e0 + M;
   }
@@ -441,6 +462,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> group_rows(
                     "n_groups must be in [1, ", kMaxGroups, "], got ",
                     n_groups);
   TORCH_CHECK_VALUE(ids_in.numel() <= kMaxRows, "too many entries");
+  check_plain("ids", ids_in);
   c10::cuda::CUDAGuard guard(ids_in.device());
   at::Tensor ids = ids_in.contiguous();
   auto opt = ids.options().dtype(at::kInt);
@@ -450,12 +472,12 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> group_rows(
   if (M == 0) return {at::zeros({G + 1}, opt), slots, order};
   at::Tensor offsets = at::empty({G + 1}, opt);
   if (ids.dtype() == at::kInt)
-    sort_launch<int>(ids.data_ptr<int>(), M, G, offsets.data_ptr<int>(),
-                     slots.data_ptr<int>(), order.data_ptr<int>(), opt);
+    sort_launch<int>(ptr<int>(ids), M, G, ptr<int>(offsets),
+                     ptr<int>(slots), ptr<int>(order), opt);
   else
-    sort_launch<int64_t>(ids.data_ptr<int64_t>(), M, G,
-                         offsets.data_ptr<int>(), slots.data_ptr<int>(),
-                         order.data_ptr<int>(), opt);
+    sort_launch<int64_t>(ptr<int64_t>(ids), M, G,
+                         ptr<int>(offsets), ptr<int>(slots),
+                         ptr<int>(order), opt);
   return {offsets, slots, order};
 }
 
@@ -759,11 +781,6 @@ unsigned row_blocks(long rows, int per) {
   return (unsigned)std::min<long>((rows + per - 1) / per, 1 << 22);
 }
 
-template <typename T>
-T* ptr(const at::Tensor& t) {
-  return reinterpret_cast<T*>(t.data_ptr());
-}
-
 // A matrix whose rows may lie apart but are contiguous in themselves.
 at::Tensor packed_rows(const at::Tensor& t) {
   if (t.size(0) == 0 || t.size(1) == 0) return t;
@@ -791,6 +808,7 @@ void check_rows(const char* name, const at::Tensor& t) {
 
 void check_ints(const char* name, const at::Tensor& t,
                 const at::Tensor& rows) {
+  check_plain(name, t);
   TORCH_CHECK_TYPE(t.dtype() == at::kInt, name, " must be int32, got ",
                    t.dtype());
   TORCH_CHECK_VALUE(t.device() == rows.device(), name, " is on ", t.device(),
@@ -834,8 +852,8 @@ at::Tensor gather_rows(const at::Tensor& x_in, const at::Tensor& offsets,
   SKA_TYPES(x.scalar_type(), [&] {
     const int lanes = lanes_for(F, Vec<T>::N), per = 256 / lanes;
     gather_kernel<T, 4><<<row_blocks(T_rows, per), 256, 0, stream_now()>>>(
-        ptr<T>(x), x.stride(0), slots.data_ptr<int>(),
-        offsets.data_ptr<int>() + offsets.numel() - 1, T_rows, k, F, lanes,
+        ptr<T>(x), x.stride(0), ptr<int>(slots),
+        ptr<int>(offsets) + offsets.numel() - 1, T_rows, k, F, lanes,
         ptr<T>(out));
     check_launch();
   });
@@ -854,10 +872,10 @@ at::Tensor combine_rows(const at::Tensor& rows_in, const at::Tensor& offsets,
   if (k == 0) return y.zero_();
   SKA_TYPES(rows.scalar_type(), [&] {
     const int lanes = lanes_for(F, Vec<T>::N), per = 256 / lanes;
-    const int* end = offsets.data_ptr<int>() + offsets.numel() - 1;
+    const int* end = ptr<int>(offsets) + offsets.numel() - 1;
     auto go = [&](auto kern, auto* w) {
       kern<<<row_blocks(T_rows, per), 256, 0, stream_now()>>>(
-          ptr<T>(rows), rows.stride(0), slots.data_ptr<int>(), end, w, T_rows,
+          ptr<T>(rows), rows.stride(0), ptr<int>(slots), end, w, T_rows,
           k, F, lanes, ptr<T>(y));
       check_launch();
     };
@@ -875,7 +893,7 @@ at::Tensor combine_rows(const at::Tensor& rows_in, const at::Tensor& offsets,
              : go(combine_kernel<T, W, 2, 2>, w);
     };
     if (!weights || weights->dtype() == at::kFloat)
-      pick(weights ? weights->data_ptr<float>() : (float*)nullptr);
+      pick(weights ? ptr<float>(*weights) : (float*)nullptr);
     else
       pick(ptr<T>(*weights));
   });
@@ -904,11 +922,11 @@ combine_rows_backward(const at::Tensor& dy_in, const at::Tensor& rows_in,
   }
   SKA_TYPES(dy.scalar_type(), [&] {
     const int lanes = lanes_for(F, Vec<T>::N), per = 256 / lanes;
-    const int* end = offsets.data_ptr<int>() + offsets.numel() - 1;
+    const int* end = ptr<int>(offsets) + offsets.numel() - 1;
     auto go = [&](auto kern, auto* w) {
       kern<<<row_blocks(T_rows, per), 256, 0, stream_now()>>>(
           ptr<T>(dy), dy.stride(0), ptr<T>(rows), rows.stride(0),
-          slots.data_ptr<int>(), end, w, T_rows, k, F, lanes,
+          ptr<int>(slots), end, w, T_rows, k, F, lanes,
           drows ? ptr<T>(*drows) : nullptr,
           dw ? ptr<std::decay_t<decltype(*w)>>(*dw) : nullptr);
       check_launch();
@@ -924,7 +942,7 @@ combine_rows_backward(const at::Tensor& dy_in, const at::Tensor& rows_in,
              : go(combine_back_kernel<T, W, 2, 2>, w);
     };
     if (!weights || weights->dtype() == at::kFloat)
-      pick(weights ? weights->data_ptr<float>() : (float*)nullptr);
+      pick(weights ? ptr<float>(*weights) : (float*)nullptr);
     else
       pick(ptr<T>(*weights));
   });
@@ -1954,11 +1972,11 @@ Parts take_parts(Product& p, at::TensorOptions opt) {
   const int64_t units = 2 * (((int64_t)p.C >> p.shift) + 1);
   if (p.out) {
     parts.part = at::empty({units, p.M, p.N}, opt.dtype(at::kFloat));
-    p.part = parts.part.data_ptr<float>();
+    p.part = ptr<float>(parts.part);
   }
   if (p.sums) {
     parts.sums = at::empty({units, p.M}, opt.dtype(at::kFloat));
-    p.part_sums = parts.sums.data_ptr<float>();
+    p.part_sums = ptr<float>(parts.sums);
   }
   return parts;
 }
@@ -2143,9 +2161,9 @@ at::Tensor product(const at::Tensor& a_in, const at::Tensor& weight,
   const int M = (int)a.size(0);
   at::Tensor out = at::empty({M, N}, a.options());
   if (out.numel() == 0) return out;
-  Product p{a.data_ptr(), weight.data_ptr(),
-            bias ? bias->data_ptr() : nullptr, out.data_ptr(), nullptr,
-            offsets.data_ptr<int>(), a.stride(0), transposed ? N : C, G, M, N,
+  Product p{ptr<void>(a), ptr<void>(weight),
+            bias ? ptr<void>(*bias) : nullptr, ptr<void>(out), nullptr,
+            ptr<int>(offsets), a.stride(0), transposed ? N : C, G, M, N,
             C, 0, nullptr, nullptr, 0, 0};
   SKA_TYPES(a.scalar_type(), [&] {
     if (transposed && C <= 16)
@@ -2192,9 +2210,9 @@ grouped_linear_dweight(const at::Tensor& dy_in, const at::Tensor& rows_in,
   if (F == 0 && !need_bias) return {dw, db};
   // rows of no width leave the bias: any other operand does for its sums
   const at::Tensor& b = F ? x : dy;
-  Product p{dy.data_ptr(), b.data_ptr(), nullptr,
-            F && dw ? dw->data_ptr() : nullptr, db ? db->data_ptr() : nullptr,
-            offsets.data_ptr<int>(), dy.stride(0), b.stride(0), G, N,
+  Product p{ptr<void>(dy), ptr<void>(b), nullptr,
+            F && dw ? ptr<void>(*dw) : nullptr, db ? ptr<void>(*db) : nullptr,
+            ptr<int>(offsets), dy.stride(0), b.stride(0), G, N,
             F ? F : N, M, 0, nullptr, nullptr, 0, 0};
   SKA_TYPES(dy.scalar_type(), [&] {
     if (sizeof(T) == 4 && N <= 16)

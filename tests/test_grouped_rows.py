@@ -1125,3 +1125,100 @@ def test_tracing_on_the_cpu_follows_its_inputs():
     traced = torch.jit.trace(run, (x, ids), check_trace=False)
     other = torch.as_tensor(ids_of("skewed", *ids.shape, G, seed=4))
     assert torch.equal(traced(x + 1, other), run(x + 1, other))
+
+
+class Wrapped(torch.Tensor):
+    """A tensor that stands for another and has no memory of its own."""
+
+    @staticmethod
+    def __new__(cls, shape, dtype):
+        return torch.Tensor._make_wrapper_subclass(cls, shape, dtype=dtype,
+                                                   device="cuda")
+
+    @classmethod
+    def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+        raise AssertionError(f"{func} was called")
+
+
+def memoryless_calls(make):
+    """Each operator with one tensor that has no memory; make(shape, dtype)
+    gives one, and real(...) an ordinary one if there is a device."""
+    f, i = torch.float32, torch.int32
+    plan = ska.GroupPlan(make((4,), i), make((3, 2), i), make((6,), i))
+    return [
+        lambda: ska.group_rows(make((3, 2), i), 3),
+        lambda: ska.gather_rows(make((3, 4), f), plan),
+        lambda: ska.combine_rows(make((6, 4), f), plan),
+        lambda: ska.combine_rows(make((6, 4), f), plan, make((3, 2), f)),
+        lambda: ska.grouped_linear(make((6, 4), f), make((3, 2, 4), f),
+                                   plan.offsets),
+    ]
+
+
+def test_refuses_tensors_without_memory():
+    """Before anything else is done with them: the device is not touched,
+    which this machine may not have."""
+    from spark_sklearn_amd.ops import extension_available
+
+    if not extension_available():
+        pytest.skip("the extension is not built")
+    for call in memoryless_calls(Wrapped):
+        with pytest.raises(TypeError, match="memory"):
+            call()
+
+
+@pytest.mark.gpu
+def test_refuses_tensors_without_memory_beside_real_ones():
+    x, ids, weight, bias, w, dy = chain_data("cuda", T=20)
+    plan = ska.group_rows(ids, weight.shape[0])
+    rows = ska.gather_rows(x, plan)
+    out = ska.grouped_linear(rows, weight, plan.offsets, bias)
+
+    def without(t):
+        return Wrapped(t.shape, t.dtype)
+
+    def zeros(t):
+        return torch._efficientzerotensor(t.shape, device="cuda")
+
+    calls = memoryless_calls(Wrapped) + [
+        lambda: ska.gather_rows(x, plan._replace(slots=without(plan.slots))),
+        lambda: ska.gather_rows(x, plan._replace(
+            offsets=without(plan.offsets))),
+        lambda: ska.gather_rows(zeros(x), plan),
+        lambda: ska.combine_rows(out, plan, without(w)),
+        lambda: ska.combine_rows(out, plan, zeros(w)),
+        lambda: ska.combine_rows(zeros(out), plan, w),
+        lambda: ska.grouped_linear(zeros(rows), weight, plan.offsets),
+        lambda: ska.grouped_linear(rows, without(weight), plan.offsets),
+        lambda: ska.grouped_linear(rows, zeros(weight), plan.offsets),
+        lambda: ska.grouped_linear(rows, weight, without(plan.offsets)),
+        lambda: ska.grouped_linear(rows, weight, plan.offsets,
+                                   without(bias)),
+        lambda: ska.grouped_linear(rows, weight, plan.offsets, zeros(bias)),
+    ]
+    for call in calls:
+        with pytest.raises(TypeError, match="memory"):
+            call()
+
+
+@pytest.mark.gpu
+def test_refuses_under_a_mode_that_makes_fake_outputs():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    x, ids, weight, bias, w, dy = chain_data("cuda", T=20)
+    plan = ska.group_rows(ids, weight.shape[0])
+    rows = ska.gather_rows(x, plan)
+    want = ska.grouped_linear(rows, weight, plan.offsets, bias)
+    many = torch.zeros(5000, dtype=torch.int64, device="cuda")
+    with FakeTensorMode(allow_non_fake_inputs=True):
+        for call in (lambda: ska.group_rows(ids, 9),
+                     lambda: ska.group_rows(many, 9),
+                     lambda: ska.gather_rows(x, plan),
+                     lambda: ska.combine_rows(rows, plan, w),
+                     lambda: ska.grouped_linear(rows, weight, plan.offsets)):
+            with pytest.raises(TypeError, match="memory"):
+                call()
+    with pytest.raises(TypeError, match="memory"):
+        torch.func.functionalize(lambda v: ska.gather_rows(v, plan))(x)
+    assert torch.equal(
+        ska.grouped_linear(rows, weight, plan.offsets, bias), want)
