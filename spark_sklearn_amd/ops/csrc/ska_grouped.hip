@@ -59,6 +59,14 @@ T* ptr(const at::Tensor& t) {
   return reinterpret_cast<T*>(t.data_ptr());
 }
 
+// A tensor's values as they lie in memory: a lazy negation (the imaginary part
+// of a conjugate has one) is carried out.
+at::Tensor as_stored(const at::Tensor& t) {
+  return t.is_neg() ? t.resolve_neg() : t;
+}
+
+at::Tensor whole(const at::Tensor& t) { return as_stored(t).contiguous(); }
+
 // The kernels have no forward-mode derivatives, and a tensor that came back
 // without its tangent would pass for a constant.
 void check_plain(const char* name, const at::Tensor& t) {
@@ -464,7 +472,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> group_rows(
   TORCH_CHECK_VALUE(ids_in.numel() <= kMaxRows, "too many entries");
   check_plain("ids", ids_in);
   c10::cuda::CUDAGuard guard(ids_in.device());
-  at::Tensor ids = ids_in.contiguous();
+  at::Tensor ids = whole(ids_in);
   auto opt = ids.options().dtype(at::kInt);
   const int M = (int)ids.numel(), G = (int)n_groups;
   at::Tensor slots = at::empty(ids.sizes(), opt);
@@ -782,7 +790,8 @@ unsigned row_blocks(long rows, int per) {
 }
 
 // A matrix whose rows may lie apart but are contiguous in themselves.
-at::Tensor packed_rows(const at::Tensor& t) {
+at::Tensor packed_rows(const at::Tensor& t_in) {
+  const at::Tensor t = as_stored(t_in);
   if (t.size(0) == 0 || t.size(1) == 0) return t;
   // the product kernels' offsets in a tile of 256 rows pass no 31 bits
   const bool fits =
@@ -837,8 +846,8 @@ Plan check_plan(const at::Tensor& rows, const at::Tensor& offsets,
   TORCH_CHECK_VALUE(slots.dim() == 1 || slots.dim() == 2,
                     "plan.slots must have one or two dimensions");
   TORCH_CHECK_VALUE(slots.numel() <= kMaxRows, "too many entries");
-  return {offsets.contiguous(),
-          (slots.dim() == 1 ? slots.unsqueeze(1) : slots).contiguous()};
+  return {whole(offsets),
+          whole(slots.dim() == 1 ? slots.unsqueeze(1) : slots)};
 }
 
 at::Tensor gather_rows(const at::Tensor& x_in, const at::Tensor& offsets,
@@ -2403,7 +2412,7 @@ at::Tensor combine_rows_checked(const at::Tensor& rows,
                       "weights must have the ids' shape ", slots.sizes(),
                       ", got ", weights->sizes());
     if (weights->dim() == 1) weights = weights->unsqueeze(1);
-    weights = weights->contiguous();
+    weights = whole(*weights);
   }
   if (!wants(rows) && !wants(weights))
     return combine_rows(rows, plan.offsets, plan.slots, weights);
@@ -2438,10 +2447,10 @@ at::Tensor grouped_linear_checked(const at::Tensor& rows,
                           bias->size(1) == N,
                       "bias must be [", G, ", ", N, "], got ",
                       bias->sizes());
-    bias = bias->contiguous();
+    bias = whole(*bias);
   }
-  const at::Tensor weight = weight_in.contiguous();
-  const at::Tensor offsets = offsets_in.contiguous();
+  const at::Tensor weight = whole(weight_in);
+  const at::Tensor offsets = whole(offsets_in);
   if (!wants(rows) && !wants(weight) && !wants(bias))
     return grouped_linear(rows, weight, offsets, bias);
   return LinearFunction::apply(rows, weight, offsets, bias, wants(rows),
@@ -2462,8 +2471,7 @@ std::tuple<Maybe, Maybe> grouped_linear_dweight_checked(
   TORCH_CHECK_VALUE(offsets.dim() == 1 && offsets.numel() >= 2 &&
                         offsets.numel() <= kMaxGroups + 1,
                     "offsets must have n_groups + 1 values");
-  return grouped_linear_dweight(dy, rows, offsets.contiguous(), need_weight,
-                                need_bias);
+  return grouped_linear_dweight(dy, rows, whole(offsets), need_weight, need_bias);
 }
 
 }  // namespace

@@ -1222,3 +1222,34 @@ def test_refuses_under_a_mode_that_makes_fake_outputs():
         torch.func.functionalize(lambda v: ska.gather_rows(v, plan))(x)
     assert torch.equal(
         ska.grouped_linear(rows, weight, plan.offsets, bias), want)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_lazily_negated_tensors(device):
+    """A tensor whose memory holds the negative of its values, as the
+    imaginary part of a conjugate does: in every place, and as a gradient."""
+    x, ids, weight, bias, w, dy = chain_data(device, T=20)
+    G = weight.shape[0]
+
+    def negated(v):
+        out = torch._neg_view(-v)
+        assert out.is_neg() and torch.equal(out, v)
+        return out
+
+    def run(make):
+        leaves = [v.clone().requires_grad_() for v in (x, weight, bias, w)]
+        a, b, c, d = (make(v) for v in leaves)
+        plan = ska.GroupPlan(*(make(v) for v in ska.group_rows(make(ids), G)))
+        out = ska.grouped_linear(ska.gather_rows(a, plan), b, plan.offsets,
+                                 c)
+        y = ska.combine_rows(out, plan, d)
+        return [y.detach()] + list(torch.autograd.grad(y, leaves, make(dy)))
+
+    for got, want in zip(run(negated), run(lambda v: v)):
+        assert torch.equal(got, want)
+    # a column of such a part, which is a matrix whose rows lie apart
+    z = torch.complex(x[:, :1], dy[:, :1]).conj().imag
+    assert z.is_neg()
+    plan = ska.group_rows(ids, G)
+    assert torch.equal(ska.gather_rows(z, plan),
+                       ska.gather_rows(-dy[:, :1], plan))
