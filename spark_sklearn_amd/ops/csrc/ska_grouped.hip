@@ -1779,7 +1779,10 @@ __global__ __launch_bounds__(256) void narrow_kernel(Product p, bool by_row) {
 // 4 columns f = 4 * (lane & 15) + e of the row (lane >> 4) * 4 + i, which are
 // four fragments' values at once.  KW of the 4 waves share the rows, the
 // others lie along f.  Bound by reading the rows: 400000 x 256 with 3 outputs
-// in 512 groups take 86 us (4.8 TB/s; 64^2 tiles 171).
+// in 512 groups take 86 us (4.8 TB/s; 64^2 tiles 171).  No accumulator takes
+// more than 512 rows: a term passes the additions of its own 512, then one for
+// each 512 rows of its wave's share, KW - 1, and one for each part of the group
+// (2048 at most).
 template <int KW>
 __global__ __launch_bounds__(256) void narrow_dweight_kernel(Product p) {
   constexpr int BF = 4 / KW * 64;
@@ -1797,37 +1800,46 @@ __global__ __launch_bounds__(256) void narrow_dweight_kernel(Product p) {
   const float* b = reinterpret_cast<const float*>(p.b) + f;
   const int n = min(r, p.M - 1);
   f32x4 acc[4] = {}, sum = {};
+  int s = seg.first + part * 16;
+  while (s < end) {
+    const int stop = ska::part_end(s, end, log2_of(KW * 512));
+    f32x4 now[4] = {}, now_sum = {};
 #pragma unroll 2
-  for (int s = seg.first + part * 16; s < end; s += KW * 16) {
-    float fa[4];
-    f32x4 fb[4];
+    for (; s < stop; s += KW * 16) {
+      float fa[4];
+      f32x4 fb[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int row = s + q * 4 + i;
-      const bool in = row < end;
-      const long at = in ? row : end - 1;
-      const float d = a[at * p.a_pitch + n];
-      fa[i] = in ? d : 0.f;
-      f32x4 v = {};
-      if (left >= 4) {
-        __builtin_memcpy(&v, b + at * p.b_pitch, 16);
-      } else {
+      for (int i = 0; i < 4; ++i) {
+        const int row = s + q * 4 + i;
+        const bool in = row < end;
+        const long at = in ? row : end - 1;
+        const float d = a[at * p.a_pitch + n];
+        fa[i] = in ? d : 0.f;
+        f32x4 v = {};
+        if (left >= 4) {
+          __builtin_memcpy(&v, b + at * p.b_pitch, 16);
+        } else {
 #pragma unroll
-        for (int e = 0; e < 3; ++e)
-          if (e < left) v[e] = b[at * p.b_pitch + e];
+          for (int e = 0; e < 3; ++e)
+            if (e < left) v[e] = b[at * p.b_pitch + e];
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) fb[i][e] = in ? v[e] : 0.f;
       }
 #pragma unroll
-      for (int e = 0; e < 4; ++e) fb[i][e] = in ? v[e] : 0.f;
+      for (int i = 0; i < 4; ++i) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          now[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(fa[i], fb[i][e],
+                                                        now[e], 0, 0, 0);
+        if (sums)
+          now_sum = __builtin_amdgcn_mfma_f32_16x16x4f32(fa[i], 1.f, now_sum,
+                                                         0, 0, 0);
+      }
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        acc[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(fa[i], fb[i][e], acc[e],
-                                                      0, 0, 0);
-      if (sums)
-        sum = __builtin_amdgcn_mfma_f32_16x16x4f32(fa[i], 1.f, sum, 0, 0, 0);
-    }
+    for (int e = 0; e < 4; ++e) acc[e] += now[e];
+    sum += now_sum;
   }
   if constexpr (KW > 1) {
     __shared__ f32x4 all[4][5][64];

@@ -1253,3 +1253,30 @@ def test_lazily_negated_tensors(device):
     plan = ska.group_rows(ids, G)
     assert torch.equal(ska.gather_rows(z, plan),
                        ska.gather_rows(-dy[:, :1], plan))
+
+
+# -- long sums ----------------------------------------------------------------
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,N,F", [
+    (1 << 24, 1, 1), (1 << 21, 3, 65), (1 << 21, 20, 8)])
+@pytest.mark.parametrize("at", [0, 12345])
+def test_no_accumulator_takes_more_than_512_rows(M, N, F, at):
+    """One term of 2^30 among ones: an accumulator of 32 bits that holds it
+    loses what is added after it, four ones at a time.  All other partial sums
+    are whole numbers of 512s below 2^25, so exact, and 2^30 and such numbers
+    add exactly (the spacing there is 128): what is lost is at most the other
+    511 rows of one accumulator."""
+    grad = torch.ones(M, N, device="cuda")
+    grad[at] = 2.0 ** 30
+    rows = torch.ones(M, F, device="cuda")
+    weight = torch.zeros(1, N, F, device="cuda", requires_grad=True)
+    bias = torch.zeros(1, N, device="cuda", requires_grad=True)
+    offsets = torch.tensor([0, M], dtype=torch.int32, device="cuda")
+    y = ska.grouped_linear(rows, weight, offsets, bias)
+    for got in torch.autograd.grad(y, [weight, bias], grad):
+        off = (got.double() - (2.0 ** 30 + M - 1)).abs().max()
+        assert float(off) <= 511
+    alone, = torch.autograd.grad(
+        ska.grouped_linear(rows, weight, offsets, bias), [bias], grad)
+    assert float((alone.double() - (2.0 ** 30 + M - 1)).abs().max()) <= 511
