@@ -1280,3 +1280,37 @@ def test_no_accumulator_takes_more_than_512_rows(M, N, F, at):
     alone, = torch.autograd.grad(
         ska.grouped_linear(rows, weight, offsets, bias), [bias], grad)
     assert float((alone.double() - (2.0 ** 30 + M - 1)).abs().max()) <= 511
+
+
+@pytest.mark.gpu
+def test_threads_on_streams_of_their_own_all_succeed():
+    """Four threads, two for each set of inputs, forward and backward: every
+    call of every thread returns, with the result it has alone."""
+    from concurrent.futures import ThreadPoolExecutor
+
+    datas = [chain_data("cuda", T=t, G=g, seed=t)
+             for t, g in ((900, 7), (2600, 21))]
+
+    def once(data):
+        x, ids, weight, bias, w, dy = data
+        leaves = [v.detach().requires_grad_() for v in (x, weight, bias, w)]
+        y = chain(leaves[0], ids, weight.shape[0], *leaves[1:])
+        return (y.detach(),) + torch.autograd.grad(y, leaves, dy)
+
+    want = [once(d) for d in datas]
+    torch.cuda.synchronize()
+
+    def work(i):
+        equal = 0
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                got = once(datas[i])
+                torch.cuda.current_stream().synchronize()
+                equal += all(torch.equal(a, b)
+                             for a, b in zip(got, want[i]))
+        return equal
+
+    with ThreadPoolExecutor(4) as pool:
+        # result() raises what a thread raised
+        done = [pool.submit(work, i) for i in (0, 1, 0, 1)]
+        assert [d.result(timeout=60) for d in done] == [20] * 4
