@@ -402,8 +402,7 @@ class KeyedModel:
         widths = np.array([len(c) for c in coefs])
         C = int(widths.max())
         coef = np.zeros((len(ests), C, X.shape[1]), np.float32)
-        # a class that a key's model does not have is never the largest
-        intercept = np.full((len(ests), C), -np.inf, np.float32)
+        intercept = np.zeros((len(ests), C), np.float32)
         for g, (e, c) in enumerate(zip(ests, coefs)):
             coef[g, :len(c)] = c
             intercept[g, :len(c)] = np.atleast_1d(e.intercept_)
@@ -415,6 +414,9 @@ class KeyedModel:
                               torch.device(device))
         out = df.copy()
         if hasattr(ests[0], "classes_"):
+            # a class that a key's model does not have is never the largest,
+            # not even where a row's scores are infinite
+            scores[np.arange(C) >= widths[row_key][:, None]] = -np.inf
             best = np.where(widths[row_key] == 1, scores[:, 0] > 0,
                             np.argmax(scores, axis=1))
             labels = np.empty((len(ests), int(best.max()) + 1), object)

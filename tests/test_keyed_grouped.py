@@ -200,3 +200,27 @@ def test_device_transform_refuses():
     wide["features"] = [np.append(v, 1.0) for v in wide["features"]]
     with pytest.raises(ValueError):
         model.transform(wide, device="cpu")
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("value", [np.inf, -np.inf, np.nan, 3e38])
+def test_device_transform_of_rows_that_are_not_finite(device, value):
+    """A key without all classes answers with one of its own, whatever the
+    row holds, as on the host."""
+    df = frame(5, 4, seed=2)
+    df.loc[(df["k"] == 3) & (df["y"] == 3), "y"] = 0      # three classes
+    df.loc[(df["k"] == 4) & (df["y"] > 1), "y"] = 0       # two
+    model = ska.KeyedEstimator(
+        sklearnEstimator=LogisticRegression(max_iter=15), keyCols=["k"],
+        yCol="y").fit(df)
+    odd = df.groupby("k").head(4).copy()
+    odd["features"] = [np.where(np.arange(9) == i % 9, value, v).astype(
+        np.float32) for i, v in enumerate(odd["features"])]
+    with np.errstate(all="ignore"):
+        host = model.transform(odd)
+        got = model.transform(odd, device=device)
+    assert got["prediction"].dtype == host["prediction"].dtype
+    known = {k: set(g["y"]) for k, g in df.groupby("k")}
+    assert all(p in known[k] for k, p in zip(got["k"], got["prediction"]))
+    if abs(value) == np.inf or np.isnan(value):
+        assert (got["prediction"] == host["prediction"]).all()
