@@ -74,15 +74,17 @@ class KeyedLinearExecutor:
                 torch.ones(1, device=self.device)
             hit = self.y == target
             t = hit.float() if loss == LOSS_LOGISTIC else \
-                torch.where(hit, 1.0, -1.0)
+                torch.where(hit, 1.0, -1.0).float()
         else:
             t = self.y
 
-        W = torch.zeros(G, C, F, device=self.device)
-        b = torch.zeros(G, C, device=self.device)
+        # the types are said, since the program may have other defaults
+        W = torch.zeros(G, C, F, dtype=torch.float32, device=self.device)
+        b = torch.zeros(G, C, dtype=torch.float32, device=self.device)
         V, Vb = torch.zeros_like(W), torch.zeros_like(b)
         active = torch.ones(G, C, dtype=torch.bool, device=self.device)
-        prev = torch.full((G, C), float("inf"), device=self.device)
+        prev = torch.full((G, C), float("inf"), dtype=torch.float32,
+                          device=self.device)
         n_iter = torch.zeros(G, C, dtype=torch.int32, device=self.device)
         k = _kernels(rows)
         for epoch in range(int(max(s["max_iter"] for s in specs))):

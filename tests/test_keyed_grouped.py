@@ -224,3 +224,34 @@ def test_device_transform_of_rows_that_are_not_finite(device, value):
     assert all(p in known[k] for k, p in zip(got["k"], got["prediction"]))
     if abs(value) == np.inf or np.isnan(value):
         assert (got["prediction"] == host["prediction"]).all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("est,n_classes", [
+    (LogisticRegression(max_iter=20), 3), (LinearSVC(max_iter=20), 2),
+    (Ridge(max_iter=20), 0)], ids=["logistic", "hinge", "ridge"])
+def test_grouped_fit_under_another_default_type(device, est, n_classes,
+                                                monkeypatch):
+    import spark_sklearn_amd.engine as engine
+
+    monkeypatch.setattr(
+        engine, "_device_or_none",
+        lambda d: torch.device(device) if device == "cuda" else None)
+    df = frame(5, n_classes, seed=6)
+
+    def fit():
+        model = ska.KeyedEstimator(sklearnEstimator=est, keyCols=["k"],
+                                   yCol="y", keySolver="grouped").fit(df)
+        scored = model.transform(df, device=device)["prediction"].to_numpy()
+        return [e.estimator.coef_ for e in
+                model.keyedModels["estimator"]] + [scored]
+
+    want = fit()
+    before = torch.get_default_dtype()
+    torch.set_default_dtype(torch.float64)
+    try:
+        got = fit()
+    finally:
+        torch.set_default_dtype(before)
+    for a, b in zip(got, want):
+        assert a.dtype == b.dtype and np.array_equal(a, b)
