@@ -41,14 +41,15 @@ def group_rows_ref(ids, n_groups):
     key = torch.where((flat >= 0) & (flat < n_groups), flat, n_groups)
     ranked, order = torch.sort(key, stable=True)
     slots = torch.empty_like(order)
-    slots[order] = torch.arange(order.numel())
-    offsets = torch.searchsorted(ranked, torch.arange(n_groups + 1))
+    slots[order] = torch.arange(order.numel(), device=ids.device)
+    offsets = torch.searchsorted(
+        ranked, torch.arange(n_groups + 1, device=ids.device))
     return offsets.int(), slots.int().reshape(ids.shape), order.int()
 
 
 def gather_rows_ref(x, offsets, slots):
     T, k = slots.shape
-    out = torch.empty(T * k, x.shape[1], dtype=x.dtype)
+    out = x.new_empty(T * k, x.shape[1])
     out[slots.long().reshape(-1)] = x.repeat_interleave(k, 0)
     out[int(offsets[-1]):] = 0
     return out
@@ -58,7 +59,7 @@ def _kept(rows, offsets, slots):
     """The rows of the kept entries [T, k, F], zero for the others."""
     kept = (slots < offsets[-1])[..., None]
     picked = _wide(rows)[slots.long()]
-    return torch.where(kept, picked, torch.zeros((), dtype=picked.dtype))
+    return torch.where(kept, picked, picked.new_zeros(()))
 
 
 def combine_rows_ref(rows, offsets, slots, weights):
@@ -78,7 +79,7 @@ def combine_rows_backward_ref(dy, rows, offsets, slots, weights, need_rows,
         spread = d[:, None].expand(T, k, d.shape[1])
         if weights is not None:
             spread = spread * weights.to(d.dtype)[..., None]
-        drows = torch.empty(T * k, dy.shape[1], dtype=dy.dtype)
+        drows = dy.new_empty(T * k, dy.shape[1])
         drows[slots.long().reshape(-1)] = spread.reshape(
             T * k, dy.shape[1]).to(dy.dtype)
         drows[int(offsets[-1]):] = 0
@@ -89,7 +90,7 @@ def combine_rows_backward_ref(dy, rows, offsets, slots, weights, need_rows,
 
 
 def grouped_linear_ref(rows, weight, offsets, bias):
-    out = torch.zeros(rows.shape[0], weight.shape[1], dtype=rows.dtype)
+    out = rows.new_zeros(rows.shape[0], weight.shape[1])
     for g, a, b in _runs(offsets):
         y = _wide(rows[a:b]) @ _wide(weight[g]).t()
         if bias is not None:
@@ -99,7 +100,7 @@ def grouped_linear_ref(rows, weight, offsets, bias):
 
 
 def grouped_linear_drows_ref(dy, weight, offsets):
-    out = torch.zeros(dy.shape[0], weight.shape[2], dtype=dy.dtype)
+    out = dy.new_zeros(dy.shape[0], weight.shape[2])
     for g, a, b in _runs(offsets):
         out[a:b] = (_wide(dy[a:b]) @ _wide(weight[g])).to(dy.dtype)
     return out
@@ -107,9 +108,8 @@ def grouped_linear_drows_ref(dy, weight, offsets):
 
 def grouped_linear_dweight_ref(dy, rows, offsets, need_weight, need_bias):
     G = offsets.numel() - 1
-    dw = torch.zeros(G, dy.shape[1], rows.shape[1],
-                     dtype=dy.dtype) if need_weight else None
-    db = torch.zeros(G, dy.shape[1], dtype=dy.dtype) if need_bias else None
+    dw = dy.new_zeros(G, dy.shape[1], rows.shape[1]) if need_weight else None
+    db = dy.new_zeros(G, dy.shape[1]) if need_bias else None
     for g, a, b in _runs(offsets):
         d = _wide(dy[a:b])
         if need_weight:

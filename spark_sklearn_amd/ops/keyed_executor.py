@@ -18,6 +18,16 @@ from ..grouped_rows import (_kernels, combine_rows, gather_rows, group_rows,
 __all__ = ["KeyedLinearExecutor", "keyed_scores"]
 
 
+def _tensor(array, dtype):
+    """On the CPU, whatever the program's default device is; a copy only if
+    the array is not writable, of another type or not contiguous."""
+    import torch
+
+    array = np.ascontiguousarray(array, dtype)
+    return torch.from_numpy(array if array.flags.writeable
+                            else array.copy())
+
+
 def _sums(values, offsets):
     """The sum of each group's run of rows [G, C]."""
     _, total = _kernels(values).grouped_linear_dweight(
@@ -34,13 +44,12 @@ class KeyedLinearExecutor:
         self.torch = torch
         self.device = torch.device("cpu") if device is None else device
         self.n_keys = n_keys
-        ids = torch.as_tensor(np.asarray(row_key, np.int64)).to(self.device)
+        ids = _tensor(row_key, np.int64).to(self.device)
         self.plan = group_rows(ids, n_keys)
-        x = torch.as_tensor(np.ascontiguousarray(X, np.float32))
+        x = _tensor(X, np.float32)
         self.rows = gather_rows(x.to(self.device), self.plan)
         self.y = gather_rows(
-            torch.as_tensor(np.asarray(y, np.float32))[:, None].to(
-                self.device), self.plan)
+            _tensor(y, np.float32)[:, None].to(self.device), self.plan)
         counts = np.bincount(row_key, minlength=n_keys)
         self.counts = counts
         sq = np.sum(np.asarray(X, np.float32).astype(np.float64) ** 2, axis=1)
@@ -65,9 +74,8 @@ class KeyedLinearExecutor:
         momentum, tol = per_key("momentum"), per_key("tol")
         limit = per_key("max_iter", torch.int32)
         intercept = per_key("fit_intercept")
-        inv_n = torch.as_tensor(
-            (1.0 / np.maximum(self.counts, 1)).astype(np.float32)).to(
-                self.device)[:, None]
+        inv_n = _tensor(1.0 / np.maximum(self.counts, 1), np.float32).to(
+            self.device)[:, None]
         loss = specs[0]["loss"]
         if n_classes:
             target = torch.arange(C, device=self.device) if C > 1 else \
@@ -126,13 +134,10 @@ class KeyedLinearExecutor:
 def keyed_scores(X, row_key, coef, intercept, device):
     """Each row's scores [n, C] under its own key's ``coef`` [G, C, F] and
     ``intercept`` [G, C]; a row whose key is outside the models scores 0."""
-    import torch
-
-    x = torch.as_tensor(np.ascontiguousarray(X, np.float32)).to(device)
-    ids = torch.as_tensor(np.asarray(row_key, np.int64)).to(device)
-    w = torch.as_tensor(np.ascontiguousarray(coef, np.float32)).to(device)
-    b = torch.as_tensor(np.ascontiguousarray(intercept,
-                                             np.float32)).to(device)
+    x = _tensor(X, np.float32).to(device)
+    ids = _tensor(row_key, np.int64).to(device)
+    w = _tensor(coef, np.float32).to(device)
+    b = _tensor(intercept, np.float32).to(device)
     plan = group_rows(ids, w.shape[0])
     out = grouped_linear(gather_rows(x, plan), w, plan.offsets, b)
     return combine_rows(out, plan).cpu().numpy()

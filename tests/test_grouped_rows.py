@@ -1314,3 +1314,18 @@ def test_threads_on_streams_of_their_own_all_succeed():
         # result() raises what a thread raised
         done = [pool.submit(work, i) for i in (0, 1, 0, 1)]
         assert [d.result(timeout=60) for d in done] == [20] * 4
+
+
+def test_the_reference_stays_on_its_tensors_device():
+    """Whatever the program's default device is."""
+    x, ids, weight, bias, w, dy = chain_data("cpu", T=20)
+
+    def run():
+        leaves = [v.detach().requires_grad_() for v in (x, weight, bias, w)]
+        y = chain(leaves[0], ids, weight.shape[0], *leaves[1:])
+        return [y.detach()] + list(torch.autograd.grad(y, leaves, dy))
+
+    want = run()
+    with torch.device("meta"):
+        got = run()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))

@@ -255,3 +255,25 @@ def test_grouped_fit_under_another_default_type(device, est, n_classes,
         torch.set_default_dtype(before)
     for a, b in zip(got, want):
         assert a.dtype == b.dtype and np.array_equal(a, b)
+
+
+@pytest.mark.parametrize("default", ["meta", pytest.param(
+    "cuda", marks=pytest.mark.gpu)])
+def test_grouped_fit_under_another_default_device(default, monkeypatch):
+    import spark_sklearn_amd.engine as engine
+
+    monkeypatch.setattr(engine, "_device_or_none", lambda d: None)
+    df = frame(4, 3, seed=6)
+
+    def fit():
+        model = ska.KeyedEstimator(
+            sklearnEstimator=LogisticRegression(max_iter=9), keyCols=["k"],
+            yCol="y", keySolver="grouped").fit(df)
+        scored = model.transform(df, device="cpu")["prediction"].to_numpy()
+        return [e.estimator.coef_ for e in
+                model.keyedModels["estimator"]] + [scored]
+
+    want = fit()
+    with torch.device(default):
+        got = fit()
+    assert all(np.array_equal(a, b) for a, b in zip(got, want))
