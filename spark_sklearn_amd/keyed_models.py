@@ -93,6 +93,8 @@ class KeyedEstimator:
     and keys that lack some of the classes to the host, one key at a time.
     """
 
+    keySolver = "columns"       # of estimators pickled without the attribute
+
     def __init__(self, sklearnEstimator=None, keyCols: Optional[List[str]] = None,
                  xCol: str = "features", yCol: Optional[str] = None,
                  estimatorType: Optional[str] = None,

@@ -277,3 +277,15 @@ def test_grouped_fit_under_another_default_device(default, monkeypatch):
     with torch.device(default):
         got = fit()
     assert all(np.array_equal(a, b) for a, b in zip(got, want))
+
+
+def test_an_estimator_pickled_without_a_key_solver_fits():
+    """As one that was saved before there was a choice."""
+    import pickle
+
+    est = ska.KeyedEstimator(sklearnEstimator=Ridge(max_iter=3),
+                             keyCols=["k"], yCol="y")
+    del est.keySolver
+    est = pickle.loads(pickle.dumps(est))
+    assert "keySolver" not in vars(est)
+    assert len(est.fit(frame(3, 0)).keyedModels) == 3
