@@ -606,7 +606,7 @@ __global__ __launch_bounds__(256) void gather_kernel(
 }
 
 // y[t] = sum over the kept entries of w[t, j] * rows[slots[t, j]], in the
-// order of j and in 32 bits; J rows are read at a time.
+// order of j and in 32 bits, rounded once; J rows are read at a time.
 template <typename T, typename W, int J, int U>
 __global__ __launch_bounds__(256) void combine_kernel(
     const T* __restrict__ rows, long pitch, const int* __restrict__ slots,
@@ -671,7 +671,8 @@ __global__ __launch_bounds__(256) void combine_kernel(
 
 // Backward of combine, in row order: dy[t] is read once for J rows, each row
 // once; drows (where asked for) and the dot products leave with them.  Bound by
-// memory: 8191 x 2 rows of 1001 float16 take 20 us (4.1 TB/s).
+// memory: 8191 x 2 rows of 1001 float16 take 20 us (4.1 TB/s).  The products
+// w * dy are rounded to the rows' type, the type that a gradient of rows has.
 template <typename T, typename W, int J, int U>
 __global__ __launch_bounds__(256) void combine_back_kernel(
     const T* __restrict__ dy, long dy_pitch, const T* __restrict__ rows,
@@ -1058,6 +1059,11 @@ __host__ __device__ constexpr int log2_of(int v) {
 //
 // The matrix instruction gets B first: a lane then holds 4 neighbouring n of
 // one m, and stores them together.
+//
+// Sums leave in their operands' type, rounded once: 32-bit outputs of 16-bit
+// operands would double the bytes that the next call reads, which bound most
+// calls, for what a caller with 16-bit tensors rounds away anyhow.  A gradient
+// through three calls carries three such roundings.
 // ---------------------------------------------------------------------------
 enum Mode { kForward, kDRows, kDWeight };
 
@@ -1378,8 +1384,8 @@ __device__ __forceinline__ bool find_job(const Product& p, int tile,
 // last tiles are half empty and 1160 tiles take five rounds of 256 CUs, not
 // 4.5. What it took from there on: loads spread among the matrix instructions
 // (1166 -> 1067 us at 8192^3; all at once they hold up the waves) and the
-// bands of find_job (-> 895: half of the L2 reads had missed).  What did not
-// help: four waves with fragments of two half steps (797 TFLOP/s), waves that
+// bands of find_job (-> 895; at 65536 x 2048 x 1024 65% of the L2's reads now
+// hit).  What did not help: four waves with fragments of two half steps (797 TFLOP/s), waves that
 // take turns at LDS and the matrix unit (708), three tiles in LDS, one block a
 // CU that goes through many tiles.
 //
