@@ -12,6 +12,7 @@
 
 #include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
+#include <ATen/EmptyTensor.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <hip/hip_runtime.h>
@@ -42,12 +43,19 @@ constexpr int64_t kMaxRows = (1ll << 31) - (1 << 16) - 1;
 
 // Whether the kernels can read a tensor: subclasses that wrap others, fake
 // tensors and zeros that are only noted as such have no memory behind them,
-// and what lies behind a functional tensor may be out of date.
+// and what lies behind a functional tensor may be out of date.  The storage is
+// looked at, since a view's pointer is not null where its storage's is, and a
+// storage may have been made smaller than its tensor (freed parameters).
 bool has_memory(const at::Tensor& t) {
-  return t.numel() == 0 ||
-         (t.layout() == at::kStrided && t.has_storage() &&
-          !t.key_set().has(c10::DispatchKey::Functionalize) &&
-          t.const_data_ptr() != nullptr);
+  if (t.numel() == 0) return true;
+  if (t.layout() != at::kStrided || !t.has_storage() ||
+      t.key_set().has(c10::DispatchKey::Functionalize))
+    return false;
+  const c10::Storage& storage = t.storage();
+  return storage.data() != nullptr &&
+         at::detail::computeStorageNbytes(t.sizes(), t.strides(),
+                                          t.itemsize(), t.storage_offset()) <=
+             storage.nbytes();
 }
 
 // No address goes to a kernel but through here.  Inputs are checked on entry;

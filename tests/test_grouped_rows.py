@@ -1329,3 +1329,63 @@ def test_the_reference_stays_on_its_tensors_device():
     with torch.device("meta"):
         got = run()
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+class WrappedView(Wrapped):
+    """The same as a view that begins behind its storage's first values: its
+    pointer is not null."""
+
+    @staticmethod
+    def __new__(cls, shape, dtype):
+        strides = [1] * len(shape)
+        for i in range(len(shape) - 1, 0, -1):
+            strides[i - 1] = strides[i] * shape[i]
+        return torch.Tensor._make_wrapper_subclass(
+            cls, shape, strides, 8, dtype=dtype, device="cuda")
+
+
+def test_refuses_views_without_memory():
+    from spark_sklearn_amd.ops import extension_available
+
+    if not extension_available():
+        pytest.skip("the extension is not built")
+    for call in memoryless_calls(WrappedView):
+        with pytest.raises(TypeError, match="memory"):
+            call()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("left", [0, 64])
+def test_refuses_tensors_whose_storage_was_given_back(left):
+    """A storage made smaller than the tensor (all of it, or all but 64
+    bytes), as freed parameters have; the tensor itself and a view."""
+    x, ids, weight, bias, w, dy = chain_data("cuda", T=20)
+    plan = ska.group_rows(ids, weight.shape[0])
+    rows = ska.gather_rows(x, plan)
+    out = ska.grouped_linear(rows, weight, plan.offsets, bias)
+
+    def freed(v, view):
+        if view:
+            v = torch.cat([v.reshape(-1)[:8], v.reshape(-1)])[8:].view(
+                v.shape)
+        else:
+            v = v.clone()
+        v.untyped_storage().resize_(left)
+        return v
+
+    for view in (False, True):
+        for call in (
+                lambda: ska.group_rows(freed(ids, view), 9),
+                lambda: ska.gather_rows(freed(x, view), plan),
+                lambda: ska.gather_rows(x, plan._replace(
+                    slots=freed(plan.slots, view))),
+                lambda: ska.combine_rows(freed(out, view), plan, w),
+                lambda: ska.combine_rows(out, plan, freed(w, view)),
+                lambda: ska.grouped_linear(freed(rows, view), weight,
+                                           plan.offsets),
+                lambda: ska.grouped_linear(rows, freed(weight, view),
+                                           plan.offsets),
+                lambda: ska.grouped_linear(rows, weight, plan.offsets,
+                                           freed(bias, view))):
+            with pytest.raises(TypeError, match="memory"):
+                call()
