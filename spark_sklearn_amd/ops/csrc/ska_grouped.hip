@@ -76,10 +76,12 @@ at::Tensor as_stored(const at::Tensor& t) {
 at::Tensor whole(const at::Tensor& t) { return as_stored(t).contiguous(); }
 
 // The kernels have no forward-mode derivatives, and a tensor that came back
-// without its tangent would pass for a constant.
+// without its tangent would pass for a constant.  (A meta tensor is on another
+// device, which the checks of devices say.)
 void check_plain(const char* name, const at::Tensor& t) {
-  TORCH_CHECK_TYPE(has_memory(t), name, " must be a tensor with memory of its "
-                   "own (no wrapper or fake tensor, dense)");
+  TORCH_CHECK_TYPE(t.is_meta() || has_memory(t), name,
+                   " must be a tensor with memory of its own (no wrapper or "
+                   "fake tensor, dense)");
   TORCH_CHECK_NOT_IMPLEMENTED(!t._fw_grad(/*level=*/0).defined(), name,
                               " has a tangent: grouped-row operators have no "
                               "forward-mode derivatives");
@@ -811,8 +813,8 @@ at::Tensor packed_rows(const at::Tensor& t_in) {
 }
 
 void check_rows(const char* name, const at::Tensor& t) {
-  check_plain(name, t);
   TORCH_CHECK_VALUE(t.is_cuda(), name, " must be on a GPU, got ", t.device());
+  check_plain(name, t);
   TORCH_CHECK_TYPE(t.dtype() == at::kFloat || t.dtype() == at::kBFloat16 ||
                        t.dtype() == at::kHalf,
                    name, " must be float32, bfloat16 or float16, got ",
@@ -1393,9 +1395,9 @@ __device__ __forceinline__ bool find_job(const Product& p, int tile,
 // 4.5. What it took from there on: loads spread among the matrix instructions
 // (1166 -> 1067 us at 8192^3; all at once they hold up the waves) and the
 // bands of find_job (-> 895; at 65536 x 2048 x 1024 65% of the L2's reads now
-// hit).  What did not help: four waves with fragments of two half steps (797 TFLOP/s), waves that
-// take turns at LDS and the matrix unit (708), three tiles in LDS, one block a
-// CU that goes through many tiles.
+// hit).  What did not help: four waves with fragments of two half steps (797
+// TFLOP/s), waves that take turns at LDS and the matrix unit (708), three tiles
+// in LDS, one block a CU that goes through many tiles.
 //
 // Tiles of c in LDS, filled by loads that write it (ASYNC) or through
 // registers: two, or one (not AHEAD) for short contractions, whose blocks hide
@@ -2497,7 +2499,8 @@ std::tuple<Maybe, Maybe> grouped_linear_dweight_checked(
   TORCH_CHECK_VALUE(offsets.dim() == 1 && offsets.numel() >= 2 &&
                         offsets.numel() <= kMaxGroups + 1,
                     "offsets must have n_groups + 1 values");
-  return grouped_linear_dweight(dy, rows, whole(offsets), need_weight, need_bias);
+  return grouped_linear_dweight(dy, rows, whole(offsets), need_weight,
+                                need_bias);
 }
 
 }  // namespace

@@ -1389,3 +1389,29 @@ def test_refuses_tensors_whose_storage_was_given_back(left):
                                            freed(bias, view))):
             with pytest.raises(TypeError, match="memory"):
                 call()
+
+
+@pytest.mark.gpu
+def test_refuses_meta_tensors_the_same_on_the_gpu():
+    """Beside tensors of either device they are on another one: ValueError."""
+    ids, plan, x, rows, weight = small()
+    bias, w = torch.ones(3, 2), torch.ones(3, 2)
+
+    def meta(v):
+        return v.to("meta")
+
+    for c in (lambda v: v, lambda v: v.cuda()):
+        p = ska.GroupPlan(*(c(v) for v in plan))
+        for call in (
+                lambda: ska.gather_rows(c(x), p._replace(
+                    slots=meta(p.slots))),
+                lambda: ska.gather_rows(c(x), p._replace(
+                    offsets=meta(p.offsets))),
+                lambda: ska.combine_rows(c(rows), p, meta(w)),
+                lambda: ska.grouped_linear(c(rows), meta(weight), p.offsets),
+                lambda: ska.grouped_linear(c(rows), c(weight),
+                                           meta(p.offsets)),
+                lambda: ska.grouped_linear(c(rows), c(weight), p.offsets,
+                                           meta(bias))):
+            with pytest.raises(ValueError):
+                call()
