@@ -428,4 +428,7 @@ class KeyedModel:
             out[self.outputCol] = list(labels[row_key, best])
         else:
             out[self.outputCol] = scores[:, 0].astype(np.float64)
-        return out.sort_index()
+        # rows of equal labels in the order in which the host's loop has them:
+        # key by key, the keys as they first appear
+        seen = pd.factorize(row_key)[0]
+        return out.iloc[np.argsort(seen, kind="stable")].sort_index()

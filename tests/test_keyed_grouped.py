@@ -289,3 +289,20 @@ def test_an_estimator_pickled_without_a_key_solver_fits():
     est = pickle.loads(pickle.dumps(est))
     assert "keySolver" not in vars(est)
     assert len(est.fit(frame(3, 0)).keyedModels) == 3
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("labels", ["same", "few", "own"])
+def test_device_transform_has_the_hosts_row_order(device, labels):
+    """Also where rows share their index label."""
+    df = frame(6, 2, seed=5)
+    model = ska.KeyedEstimator(sklearnEstimator=LogisticRegression(
+        max_iter=9), keyCols=["k"], yCol="y").fit(df)
+    df["row"] = np.arange(len(df))
+    df.loc[df.index[4], "k"] = 99
+    if labels != "own":
+        df.index = np.zeros(len(df), int) if labels == "same" else \
+            np.arange(len(df))[::-1] // 7
+    host = model.transform(df, unseenKeys="drop")
+    got = model.transform(df, unseenKeys="drop", device=device)
+    pd.testing.assert_frame_equal(got, host)
