@@ -376,12 +376,15 @@ class KeyedModel:
             # grouping by key passes over rows without one
             df = df[df[self.keyCols].notna().all(axis=1)]
 
-        def index(frame):
-            if len(self.keyCols) == 1:
-                return pd.Index(frame[self.keyCols[0]])
-            return pd.MultiIndex.from_frame(frame[self.keyCols])
-
-        row_key = index(models).get_indexer(index(df))
+        # a key is looked up as the host's loop does, once for all its rows
+        known = {key: i for i, key in enumerate(
+            zip(*(models[c] for c in self.keyCols)))}
+        code = df.groupby(self.keyCols, sort=False).ngroup().to_numpy()
+        _, first, code = np.unique(code, return_index=True,
+                                   return_inverse=True)
+        keys = list(zip(*(df[c].iloc[first] for c in self.keyCols)))
+        row_key = np.array([known.get(key, -1) for key in keys],
+                           np.int64)[code]
         if (row_key < 0).any():
             if unseenKeys == "error":
                 first = df.iloc[int(np.argmax(row_key < 0))]

@@ -306,3 +306,19 @@ def test_device_transform_has_the_hosts_row_order(device, labels):
     host = model.transform(df, unseenKeys="drop")
     got = model.transform(df, unseenKeys="drop", device=device)
     pd.testing.assert_frame_equal(got, host)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("change", [
+    lambda k: k.astype(float), lambda k: k == 1, lambda k: k.astype("Int64"),
+    lambda k: k.astype("category"), lambda k: k.astype(object),
+    lambda k: k.astype("int8")],
+    ids=["float", "bool", "nullable", "category", "object", "int8"])
+def test_device_transform_finds_the_keys_that_the_host_finds(device, change):
+    """Keys of another type that equal the models'."""
+    df = frame(2, 2, seed=9)
+    model = ska.KeyedEstimator(sklearnEstimator=LogisticRegression(
+        max_iter=9), keyCols=["k"], yCol="y").fit(df)
+    df["k"] = change(df["k"])
+    pd.testing.assert_frame_equal(model.transform(df, device=device),
+                                  model.transform(df))
